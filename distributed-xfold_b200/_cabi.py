@@ -71,6 +71,12 @@ class DiffusionWeights(C.Structure):
                 ("ln_cond", vp)]
 
 
+class QkNorm(C.Structure):
+    _fields_ = [(n, ci) for n in ("B", "S", "Hq", "Hk", "D", "rot", "neighbours", "is_f32")] + \
+               [(n, vp) for n in ("q_weight", "k_weight", "freqs", "positions")] + \
+               [("pos_batch_stride", ll), ("eps", cf), ("q_scale", cf)]
+
+
 class ShardDesc(C.Structure):
     _fields_ = [("world", ci), ("rank", ci), ("n_tokens", ci), ("row_starts", C.POINTER(ci)),
                 ("zbuf0", C.POINTER(vp)), ("zbuf1", C.POINTER(vp)), ("plane_a", C.POINTER(vp)), ("plane_b", C.POINTER(vp)),
@@ -134,6 +140,12 @@ SIGNATURES = {
     "xfold_grid_attention_fwd": (ci, [vp, vp, ci, ci, ci, ci, vp, vp, vp, vp, ll, vp, ci, vp, ci, vp, sz, vp]),
     "xfold_diffusion_workspace_bytes": (sz, [ci, ci, C.POINTER(DiffusionWeights)]),
     "xfold_diffusion_transformer_fwd": (ci, [vp, vp, ci, ci, vp, vp, C.POINTER(DiffusionWeights), C.POINTER(vp), vp, sz, vp]),
+    "xfold_relative_bias_fwd": (ci, [vp, vp, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, ci, vp, vp]),
+    "xfold_relative_bias_bwd_workspace_bytes": (sz, [vp, ci, ci, ci, ci]),
+    "xfold_relative_bias_bwd": (ci, [vp, vp, ci, ll, ll, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, vp, vp, sz, vp]),
+    "xfold_qk_norm_rotate_fwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 4 + [vp]),
+    "xfold_qk_norm_rotate_bwd_workspace_bytes": (sz, [vp, ci]),
+    "xfold_qk_norm_rotate_bwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 6 + [vp, vp, vp, sz, vp]),
     "xfold_cross_attention_workspace_bytes": (sz, [ci, ci, ci, ci, ci]),
     "xfold_cross_attention_fwd": (ci, [vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "xfold_pairformer_f32_workspace_bytes": (sz, [ci]),

@@ -247,6 +247,53 @@ int xfold_cross_attention_fwd(xfold_ctx* ctx, const void* q_data, const void* m_
                               int H, int D, const void* w_qg, const float* qg_bias, const float* qg_scale,
                               const void* w_kv, const float* bias, void* out, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- positions in attention (no counterpart in the reference) ---------------------------------------
+ * A learned bias of the logits by buckets of relative position:
+ *   out[h][i][j] = table[b(i, j)][h],  b(i, j) = buckets[clamp(k_pos[j] - q_pos[i], -reach, reach) + reach],
+ * or the table's last row where q_group[i] != k_group[j] (both groups or neither; tokens of different chains).
+ *   table float32 [num_buckets][H]; buckets int32 [2 * reach + 1], rows of the table (one that names none makes its entries
+ *   not a number); positions and groups int32; num_buckets <= 1024, reach <= 4096.
+ *   form: float32 or bf16 [H][Sq][Sk], or the prepared pair bias of the attention core, float16 [H][Sq][pad8(Sk)] times
+ *   log2(e) within +-60000, zero behind the last key (what is not a number: -60000). */
+enum { XFOLD_BIAS_F32 = 0, XFOLD_BIAS_BF16 = 1, XFOLD_BIAS_PREPARED = 2 };
+int xfold_relative_bias_fwd(xfold_ctx* ctx, const float* table, int num_buckets, int H, const int* buckets, int reach,
+                            const int* q_pos, const int* k_pos, const int* q_group, const int* k_group, int Sq, int Sk,
+                            int form, void* out, void* stream);
+/* Gradient of the table: dtable[b][h] = sum over (i, j) with b(i, j) = b of grad[h][i][j]; float32 [num_buckets][H],
+ * overwritten.  grad float32 or bf16, element (h, i, j) at h * head_stride + i * query_stride + j.  (Entries whose bucket
+ * names no row are left out.)  The sums' order is fixed: the same call gives the same bits. */
+size_t xfold_relative_bias_bwd_workspace_bytes(xfold_ctx* ctx, int num_buckets, int H, int Sq, int Sk);
+int xfold_relative_bias_bwd(xfold_ctx* ctx, const void* grad, int is_f32, long long head_stride, long long query_stride,
+                            int num_buckets, int H, const int* buckets, int reach, const int* q_pos, const int* k_pos,
+                            const int* q_group, const int* k_group, int Sq, int Sk, float* dtable, void* ws,
+                            size_t ws_bytes, void* stream);
+
+/* Norms of queries and keys for each head, and their rotation by position:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight (* q_scale for queries); of the first `rot` elements of a head the pairs (a, b),
+ *   (i, i + rot / 2) or neighbours (2 i, 2 i + 1), become (a cos t - b sin t, b cos t + a sin t), t = position * freqs[i].
+ * Heads of D <= 256 elements (even); batch, token and head strides in elements, so that q and k may lie in the result of a
+ * fused projection; results may lie over their inputs.  weights float32 [D] or NULL (ones); freqs float64 [rot / 2] on the
+ * device; positions int32, that of token s of batch entry b at b * pos_batch_stride + s, or NULL (s).  bf16 or float32. */
+typedef struct {
+  int B, S, Hq, Hk, D, rot, neighbours, is_f32;
+  const float *q_weight, *k_weight;
+  const double* freqs;
+  const int* positions;
+  long long pos_batch_stride;
+  float eps, q_scale;
+} xfold_qk_norm;
+int xfold_qk_norm_rotate_fwd(xfold_ctx* ctx, const xfold_qk_norm* n, const void* q, const long long q_strides[3], const void* k,
+                             const long long k_strides[3], void* q_out, const long long q_out_strides[3], void* k_out,
+                             const long long k_out_strides[3], void* stream);
+/* dq, dk (over the gradients of the results, dq_out and dk_out, if wished) and the weights' gradients, float32 [D], summed in a
+ * fixed order (NULL: not wanted); q and k are the forward's inputs. */
+size_t xfold_qk_norm_rotate_bwd_workspace_bytes(xfold_ctx* ctx, int D);
+int xfold_qk_norm_rotate_bwd(xfold_ctx* ctx, const xfold_qk_norm* n, const void* dq_out, const long long dq_out_strides[3],
+                             const void* dk_out, const long long dk_out_strides[3], const void* q, const long long q_strides[3],
+                             const void* k, const long long k_strides[3], void* dq, const long long dq_strides[3], void* dk,
+                             const long long dk_strides[3], float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes,
+                             void* stream);
+
 /* ---- PairformerBlock --------------------------------------------------------------------------
  * DistributePairformerBlock.forward (nn/d_pairformer.py:99-171) for world size 1: both TriMuls,
  * both TriAttns, pair Transition, then pair-logit projection, single AttentionPairBias (16 heads x 24,
