@@ -4,4 +4,4 @@ import it through ``__graft_entry__.load_package()`` (registers it as ``distribu
 """
 from . import _cabi  # noqa: F401
 
-__all__ = ["_cabi", "ops", "position_ops"]
+__all__ = ["_cabi", "ops", "position_ops", "int8_ops"]

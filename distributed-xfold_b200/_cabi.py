@@ -146,6 +146,10 @@ SIGNATURES = {
     "xfold_qk_norm_rotate_fwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 4 + [vp]),
     "xfold_qk_norm_rotate_bwd_workspace_bytes": (sz, [vp, ci]),
     "xfold_qk_norm_rotate_bwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 6 + [vp, vp, vp, sz, vp]),
+    "xfold_quantize_rows_fwd": (ci, [vp, vp, ci, ll, ll, ci, vp, ll, vp, vp]),
+    "xfold_linear_int8_quantized_fwd": (ci, [vp, vp, ll, vp, ll, ci, vp, ll, ci, vp, vp, vp, ci, ll, vp]),
+    "xfold_linear_int8_workspace_bytes": (sz, [ll, ci]),
+    "xfold_linear_int8_fwd": (ci, [vp, vp, ci, ll, ll, ci, vp, ll, ci, vp, vp, vp, ci, ll, vp, sz, vp]),
     "xfold_cross_attention_workspace_bytes": (sz, [ci, ci, ci, ci, ci]),
     "xfold_cross_attention_fwd": (ci, [vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
     "xfold_pairformer_f32_workspace_bytes": (sz, [ci]),

@@ -9,10 +9,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["api.cu", "gemm.cu", "gemm_split.cu", "simt.cu", "attention.cu", "peer.cu", "sharded.cu", "fp32_validation.cu", "cross_attention.cu", "pair_logits.cu",
            "diffusion.cu", "transition.cu", "row_project.cu",
-           "row_output.cu", "position.cu"]
+           "row_output.cu", "position.cu", "int8.cu"]
 # the fp32 validation kernels want IEEE division, exact exponentials and denormals, the position kernels float32 results
-# and exact angles: no fast-math for these files
-NO_FAST_MATH = {"fp32_validation.cu", "position.cu"}
+# and exact angles, the 8-bit kernels exact quotients: no fast-math for these files
+NO_FAST_MATH = {"fp32_validation.cu", "position.cu", "int8.cu"}
 LIB = os.path.join(HERE, "libxfold_b200.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall", "-Xcompiler", "-Wno-unused-function"]

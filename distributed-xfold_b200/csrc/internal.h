@@ -138,6 +138,10 @@ cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), int grid, int cluster, in
 // 128-byte swizzle (64-byte for boxes whose rows are 64 bytes, 0 for none), zero fill outside the extents.
 bool make_tmap_bf16_3d(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1,
                        uint64_t s2, uint32_t b0, uint32_t b1, uint32_t b2, int swizzle_bytes = 128);
+// the same of other types
+enum TmapType : int { TMAP_U8, TMAP_BF16, TMAP_F32 };
+bool make_tmap_3d(CUtensorMap* m, TmapType type, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1, uint64_t s2,
+                  uint32_t b0, uint32_t b1, uint32_t b2, int swizzle_bytes);
 
 // ---- GEMM ---------------------------------------------------------------------------------
 // COLS: PLAIN with column vectors or columns that leave in another form.  A kernel of its own: what PLAIN does not need would

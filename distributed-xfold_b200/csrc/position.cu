@@ -777,17 +777,6 @@ static int qk_fill(Ctx* c, const xfold_qk_norm* n, QkArgs& a, const char* what) 
 
 static void qk_strides(const long long s[3], long long& b, long long& t, long long& h) { b = s[0]; t = s[1]; h = s[2]; }
 
-struct DeviceGuard {  // launches go to the context's device, whichever is the thread's own
-  int before = -1;
-  explicit DeviceGuard(const Ctx* c) {
-    int d = -1;
-    if (cudaGetDevice(&d) == cudaSuccess && d != c->device && cudaSetDevice(c->device) == cudaSuccess) before = d;
-  }
-  ~DeviceGuard() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
-
 }  // namespace xf
 
 using namespace xf;

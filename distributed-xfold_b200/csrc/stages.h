@@ -25,6 +25,17 @@ struct Carver {
   bool ok() const { return off <= cap; }
 };
 
+struct DeviceGuard {  // launches go to the context's device, whichever is the thread's own
+  int before = -1;
+  explicit DeviceGuard(const Ctx* c) {
+    int d = -1;
+    if (cudaGetDevice(&d) == cudaSuccess && d != c->device && cudaSetDevice(c->device) == cudaSuccess) before = d;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 // Lets a caller overlap what follows an operator's LAST GEMM with that GEMM: the GEMM is issued in `parts` chunks of
 // rows (chunk boundaries at multiples of `unit` rows) and `after(first_row, rows)` is called once a chunk is launched.
 // The multi-GPU block uses it to send finished rows to their next owner on a second stream while the rest computes.

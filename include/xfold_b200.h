@@ -294,6 +294,23 @@ int xfold_qk_norm_rotate_bwd(xfold_ctx* ctx, const xfold_qk_norm* n, const void*
                              const long long dk_strides[3], float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes,
                              void* stream);
 
+/* ---- linear layers in 8-bit integers (no counterpart in the reference) --------------------------------
+ * Rows to 8 bits: scale[m] = max_k |x[m][k]| / 127 in float32, q[m][k] = x[m][k] / scale[m] rounded to the nearest whole
+ * number (ties to even; exact).  x bf16 or float32; q int8, rows ldq apart, zeros from K to the next multiple of 16 (as far as
+ * ldq leaves room).  Rows whose scale would be subnormal: zeros, scale 0; rows that hold something not finite: scale NaN. */
+int xfold_quantize_rows_fwd(xfold_ctx* ctx, const void* x, int is_f32, long long ldx, long long M, int K, void* q, long long ldq,
+                            float* scale, void* stream);
+/* out[m][n] = (sum_k x[m][k] w[n][k]) * x_scale[m] * w_scale[n] + bias[n]: x and w int8, rows 16-byte aligned and ldx, ldw
+ * (multiples of 16) apart; sums in 32-bit integers, exact (K <= 131072); bias may be NULL; out bf16 or float32, any ldo >= N. */
+int xfold_linear_int8_quantized_fwd(xfold_ctx* ctx, const void* x, long long ldx, const float* x_scale, long long M, int K,
+                                    const void* w, long long ldw, int N, const float* w_scale, const float* bias, void* out,
+                                    int out_is_f32, long long ldo, void* stream);
+/* Both in one call, x bf16 or float32. */
+size_t xfold_linear_int8_workspace_bytes(long long M, int K);
+int xfold_linear_int8_fwd(xfold_ctx* ctx, const void* x, int is_f32, long long ldx, long long M, int K, const void* w, long long ldw,
+                          int N, const float* w_scale, const float* bias, void* out, int out_is_f32, long long ldo, void* ws,
+                          size_t ws_bytes, void* stream);
+
 /* ---- PairformerBlock --------------------------------------------------------------------------
  * DistributePairformerBlock.forward (nn/d_pairformer.py:99-171) for world size 1: both TriMuls,
  * both TriAttns, pair Transition, then pair-logit projection, single AttentionPairBias (16 heads x 24,

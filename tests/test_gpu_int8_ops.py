@@ -1,0 +1,241 @@
+"""GPU: linear layers in 8-bit integers against whole numbers and 64 bits.
+
+The quantised rows are whole numbers by definition: equal to x / scale in 64 bits, rounded to even (two 24-bit numbers' quotient
+is never nearer than 2^-32 to a border that it does not lie on).  The sums are exact; a result has the roundings of the sum to
+float32, of two products and of the bias' addition (u = 2^-24 each, below 4 u of |sum s w| + |bias|), then half a step of its type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+BF, F32, I8 = torch.bfloat16, torch.float32, torch.int8
+U = 2.0 ** -24
+HALF = {BF: 2.0 ** -8, F32: U}
+
+
+@pytest.fixture(scope="module")
+def Q(ops):
+    from distributed_xfold_b200 import int8_ops
+    return int8_ops
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def plain_rows(x):
+    x = x.cpu()
+    scale = x.float().abs().amax(-1) / 127
+    return torch.where(scale[..., None] > 0, x.double() / scale.double()[..., None].clamp_min(1e-300), 0.0).round(), scale
+
+
+def weights(n, k, seed):
+    w = torch.zeros(n, (k + 15) // 16 * 16, dtype=I8)
+    w[:, :k] = torch.randint(-127, 128, (n, k), generator=gen(seed)).to(I8)
+    w = w.cuda()
+    if k % 16:
+        w[:, k:] = 77   # what lies between the rows is not read as weights
+    return w[:, :k], (torch.rand(n, generator=gen(seed + 1)) + 0.5).div(k).cuda()
+
+
+def check_linear(out, q, s, w, ws, bias, dtype):
+    acc = q.reshape(-1, q.shape[-1]) @ w.cpu().double().T
+    y = acc * s.reshape(-1, 1).double() * ws.cpu().double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64) if bias is None else bias.cpu().double()
+    want, tol = y + b, 4 * U * (y.abs() + b.abs())
+    tol = tol + HALF[dtype] * (want.abs() + tol)
+    got = out.double().cpu().reshape(want.shape)
+    assert out.dtype == dtype and ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol.clamp_min(1e-300)).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 768), (3, 7), (5, 33), (130, 384), (17, 1000), (9, 1024), (4, 1032), (2, 5001), (3, 16384), (2, 40000), (1, 131072)])
+def test_quantize_rows(Q, ops, m, k, dtype):
+    x = (torch.randn(m, k, generator=gen(m + k)) * torch.logspace(-3, 3, m)[:, None]).to(dtype)
+    q, s = Q.quantize_rows(x.cuda())
+    want, scale = plain_rows(x)
+    assert q.dtype == I8 and q.stride(0) % 16 == 0 and torch.equal(s.cpu(), scale) and torch.equal(q.cpu().double(), want)
+    whole = torch.as_strided(q, (m, q.stride(0)), (q.stride(0), 1))
+    assert not whole[:, k:].any()
+    ops.synchronize_and_check()
+
+
+def test_quantize_rows_at_borders(Q):
+    """Ties, and quotients a step of the last bit away from them."""
+    half = torch.arange(-126, 126).float() + 0.5
+    near = torch.nextafter(half, torch.full_like(half, 1e9)), torch.nextafter(half, torch.full_like(half, -1e9))
+    base = torch.cat([torch.tensor([127.0]), half, *near])
+    for f in (1.0, 2.0 ** -20, 3.0, 0.1, 1e30, 1e-30):
+        x = base * f
+        q, s = Q.quantize_rows(x[None].cuda())
+        want, scale = plain_rows(x[None])
+        assert torch.equal(s.cpu(), scale) and torch.equal(q.cpu().double(), want)
+    assert torch.equal(Q.quantize_rows(base[None].cuda())[0].cpu().double()[0, 1:253], torch.round(half.double()))
+
+
+def test_quantize_rows_that_are_empty_or_not_finite(Q):
+    x = torch.zeros(6, 40)
+    x[1, 3], x[2, 5], x[3, 7], x[4, 0], x[5, 39] = float("nan"), float("inf"), -float("inf"), 1e-39, 3e38
+    for t in (x, x[:, :33].contiguous()):
+        q, s = Q.quantize_rows(t.cuda())
+        assert s[0] == 0 and s[4] == 0 and not q[:5].any()
+        assert s[1:4].isnan().tolist() == [True, True, True]
+    q, s = Q.quantize_rows(x.cuda())
+    assert q[5, 39] == 127 and s[5] == torch.tensor(3e38) / 127
+    w, ws = weights(24, 40, 3)
+    out = Q.linear_int8(x.cuda(), w, ws, dtype=F32)
+    large = (127.0 * w[:, 39].double() * s[5].double() * ws.double()).float()   # some beyond the largest float32, others not
+    assert out[1:4].isnan().all() and not out[0].any() and torch.equal(out[5].isfinite(), large.isfinite())
+
+
+LINEAR = [  # rows, inner, channels
+    (1, 1, 1), (1, 768, 4096), (2, 100, 130), (7, 16, 8), (8, 1000, 1030), (9, 512, 640), (16, 4096, 96), (17, 48, 4097), (31, 2050, 33), (64, 768, 1536),
+    (77, 384, 1536), (127, 130, 1000), (128, 128, 256), (129, 4096, 257), (300, 1536, 768), (1000, 200, 2000), (2500, 768, 1152), (700, 5000, 350)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k,n", LINEAR)
+def test_linear_int8(Q, ops, m, k, n, dtype):
+    x = torch.randn(m, k, generator=gen(m + n)).to(dtype)
+    w, ws = weights(n, k, k)
+    bias = torch.randn(n, generator=gen(7)).cuda()
+    q, s = plain_rows(x)
+    out = Q.linear_int8(x.cuda(), w, ws, bias)
+    check_linear(out, q, s, w, ws, bias, dtype)
+    other = F32 if dtype == BF else BF
+    check_linear(Q.linear_int8(x.cuda(), w, ws, dtype=other), q, s, w, ws, None, other)
+    xq, xs = Q.quantize_rows(x.cuda())
+    assert torch.equal(Q.linear_int8_quantized(xq, xs, w, ws, bias, dtype), out)
+    assert torch.equal(Q.linear_int8(x.cuda(), w, ws, bias), out)
+    ops.synchronize_and_check()
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 200])
+def test_linear_int8_with_the_largest_sums(Q, m):
+    """The longest row of largest numbers: sums of 127 * 127 * 131072, which only whole numbers hold exactly."""
+    k, n = 131072, 40
+    x = torch.full((m, k), 1.0)
+    x[:, ::3] = -1.0
+    w = torch.full((n, k), 127, dtype=I8)
+    w[1::2] = torch.where(torch.arange(k) % 3 == 0, -127, 127).to(I8)
+    ws = torch.ones(n)
+    out = Q.linear_int8(x.cuda(), w.cuda(), ws.cuda(), dtype=F32)
+    q, s = plain_rows(x)
+    check_linear(out, q, s, w, ws, None, F32)
+
+
+def test_linear_int8_of_views(Q):
+    """Rows apart, a leading axis, weights with longer rows, activations at odd elements."""
+    m, k, n = 30, 96, 72
+    base = torch.randn(2, m, k + 9, generator=gen(1)).to(BF).cuda()
+    wide = torch.randint(-127, 128, (n, 160), generator=gen(2)).to(I8).cuda()
+    w, ws = wide[:, 32:32 + k], torch.rand(n, generator=gen(3)).cuda()
+    for x in (base[0, :, :k], base[1, :, 1:k + 1], base[..., :k], base[:, ::2, 8:k + 8], base[:1, :1, :k].expand(2, 5, k), base[0, :, :k].t()[:, :24].t()):
+        out = Q.linear_int8(x, w, ws)
+        assert out.shape == (*x.shape[:-1], n)
+        q, s = plain_rows(x)
+        check_linear(out, q, s, w, ws, None, BF)
+    vec = base[0, 3, :k]
+    assert torch.equal(Q.linear_int8(vec, w, ws), Q.linear_int8(vec[None], w, ws)[0])
+
+
+def test_linear_int8_without_rows_or_channels(Q):
+    w, ws = weights(5, 32, 1)
+    assert tuple(Q.linear_int8(torch.zeros(0, 32).cuda(), w, ws).shape) == (0, 5)
+    assert tuple(Q.linear_int8(torch.zeros(2, 0, 32).cuda(), w, ws).shape) == (2, 0, 5)
+    assert tuple(Q.linear_int8(torch.zeros(3, 32).cuda(), w[:0], ws[:0]).shape) == (3, 0)
+    q, s = Q.quantize_rows(torch.zeros(0, 32).cuda())
+    assert tuple(q.shape) == (0, 32) and tuple(s.shape) == (0,)
+    assert tuple(Q.linear_int8_quantized(q, s, w, ws).shape) == (0, 5)
+
+
+def test_linear_int8_refusals_of_the_library(Q):
+    from distributed_xfold_b200._cabi import XfoldError
+    with pytest.raises(XfoldError, match="K up to 131072"):
+        Q.quantize_rows(torch.zeros(1, 131073).cuda())
+    w = torch.zeros(2, 131088, dtype=I8).cuda()
+    with pytest.raises(XfoldError, match="K up to 131072"):
+        Q.linear_int8(torch.zeros(1, 131088).cuda(), w, torch.ones(2).cuda())
+
+
+def calls(Q):
+    w, ws = weights(520, 200, 4)
+    w2, ws2 = weights(200, 520, 5)
+
+    def make(seed):
+        return (torch.randn(150, 200, generator=gen(seed)).to(BF).cuda(), torch.randn(2, 200, generator=gen(seed + 9)).to(BF).cuda())
+
+    def call(x, y):
+        outs = [Q.linear_int8(t, w, ws) for t in (x, y)]
+        return (*outs, *(Q.linear_int8(t, w2, ws2, dtype=F32) for t in outs))
+
+    return make, call
+
+
+def test_int8_calls_on_several_streams(Q):
+    make, call = calls(Q)
+    inputs = [make(s) for s in range(3)]
+    want = [[t.clone() for t in call(*x)] for x in inputs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [[] for _ in range(3)]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(call(*inputs[i]))
+    torch.cuda.synchronize()
+    for i in range(3):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_int8_calls_captured(Q, ops):
+    make, call = calls(Q)
+    static, want = make(0), [[t.clone() for t in call(*make(s))] for s in range(2)]
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for graph in graphs:
+        with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+            outs.append(call(*static))
+    ops._Workspace.release()
+    filler = torch.full((1 << 26,), 0x7F, dtype=torch.uint8, device="cuda")
+    for seed in (1, 0):
+        for dst, src in zip(static, make(seed)):
+            dst.copy_(src)
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[seed]))
+    del filler
+
+
+def test_projections_norms_and_bias_of_an_attention_layer(Q, ops):
+    """The operators in a row, as an attention layer has them: 8-bit projection to queries, keys, values and gate, norms and
+    rotation where q and k lie in it, and the prepared bias in the attention core against the same core with the bias as numbers."""
+    from distributed_xfold_b200 import position_ops as P
+    n, c, heads, d = 70, 384, 16, 24
+    g = gen(6)
+    x = torch.randn(1, n, c, generator=g).to(BF).cuda()
+    wq, ws = Q.quantize_rows((torch.randn(4 * c, c, generator=g) * c ** -0.5).cuda())
+    proj = Q.linear_int8(x, wq, ws)
+    q, s = plain_rows(x)
+    check_linear(proj, q, s, wq, ws, None, BF)
+    views = [proj[..., i * c:(i + 1) * c].unflatten(-1, (heads, d)) for i in range(2)]
+    w = [(1 + 0.1 * torch.randn(d, generator=g)).cuda() for _ in range(2)]
+    rotation, keep = P.Rotation.make(d), proj.clone()
+    want = P.norm_rotate_qk(*(v.contiguous() for v in views), *w, rotation, q_scale=d ** -0.5)
+    P.norm_rotate_qk_(*views, *w, rotation, q_scale=d ** -0.5)
+    assert torch.equal(views[0], want[0]) and torch.equal(views[1], want[1]) and torch.equal(proj[..., 2 * c:], keep[..., 2 * c:])
+    lut = torch.tensor(P.clipped_buckets(32), dtype=torch.int32).cuda()
+    chain = (torch.arange(n) // 40).int().cuda()
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    table = torch.randn(66, heads, generator=g).cuda()
+    packed = ops.PackedSelfAttention(_attention_state(g, c), "", "cuda", heads)
+    out = ops.attention_pair_bias_core(x, packed, P.relative_position_bias(table, lut, pos, None, chain, prepared=True), None)
+    ref = ops.attention_pair_bias_core(x, packed, P.relative_position_bias(table, lut, pos, None, chain), None)
+    assert torch.equal(out, ref) and out.isfinite().all()
+    ops.synchronize_and_check()
+
+
+def _attention_state(g, c):
+    st = {n + ".weight": torch.randn(c, c, generator=g) * c ** -0.5 for n in ("q_projection", "k_projection", "v_projection", "gating_query")}
+    st["adaptive_zero_init.transition2.weight"] = torch.randn(c, c, generator=g) * c ** -0.5
+    return st
