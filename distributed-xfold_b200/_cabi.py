@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from typing import Optional
 
@@ -71,10 +72,8 @@ class DiffusionWeights(C.Structure):
                 ("ln_cond", vp)]
 
 
-class QkNorm(C.Structure):
-    _fields_ = [(n, ci) for n in ("B", "S", "Hq", "Hk", "D", "rot", "neighbours", "is_f32")] + \
-               [(n, vp) for n in ("q_weight", "k_weight", "freqs", "positions")] + \
-               [("pos_batch_stride", ll), ("eps", cf), ("q_scale", cf)]
+# xfold_qk_norm, packed by the call: a struct of this size is made several times faster so than by field
+QK_NORM = struct.Struct("8i4Pqff" + "P3q" * 6)
 
 
 class ShardDesc(C.Structure):
@@ -143,9 +142,9 @@ SIGNATURES = {
     "xfold_relative_bias_fwd": (ci, [vp, vp, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, ci, vp, vp]),
     "xfold_relative_bias_bwd_workspace_bytes": (sz, [vp, ci, ci, ci, ci]),
     "xfold_relative_bias_bwd": (ci, [vp, vp, ci, ll, ll, ci, ci, vp, ci, vp, vp, vp, vp, ci, ci, vp, vp, sz, vp]),
-    "xfold_qk_norm_rotate_fwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 4 + [vp]),
+    "xfold_qk_norm_rotate_fwd": (ci, [vp, C.c_char_p, vp]),
     "xfold_qk_norm_rotate_bwd_workspace_bytes": (sz, [vp, ci]),
-    "xfold_qk_norm_rotate_bwd": (ci, [vp, C.POINTER(QkNorm)] + [vp, C.POINTER(ll)] * 6 + [vp, vp, vp, sz, vp]),
+    "xfold_qk_norm_rotate_bwd": (ci, [vp, C.c_char_p, vp, vp, vp, sz, vp]),
     "xfold_quantize_rows_fwd": (ci, [vp, vp, ci, ll, ll, ci, vp, ll, vp, vp]),
     "xfold_linear_int8_quantized_fwd": (ci, [vp, vp, ll, vp, ll, ci, vp, ll, ci, vp, vp, vp, ci, ll, vp]),
     "xfold_linear_int8_workspace_bytes": (sz, [ll, ci]),

@@ -755,7 +755,8 @@ static int launch_qk(Ctx* c, QkArgs a, int f32, int neighbours, cudaStream_t st,
   return check_launch(c, "qk_weight_grad_kernel");
 }
 
-static int qk_fill(Ctx* c, const xfold_qk_norm* n, QkArgs& a, const char* what) {
+// the call's description as the kernels take it
+static int qk_fill(Ctx* c, const xfold_qk_norm* n, QkArgs& a, bool grad, const char* what) {
   if (!n) return fail(c, XFOLD_ERR_ARG, "%s: null argument", what);
   if (n->B < 0 || n->S < 0 || n->Hq < 0 || n->Hk < 0 || n->D < 2 || n->D > 256 || n->D % 2)
     return fail(c, XFOLD_ERR_ARG, "%s: sizes (heads of an even width up to 256)", what);
@@ -766,16 +767,21 @@ static int qk_fill(Ctx* c, const xfold_qk_norm* n, QkArgs& a, const char* what) 
   a.B = n->B; a.S = n->S; a.D = n->D; a.rot = n->rot;
   a.freqs = n->freqs; a.pos = n->positions; a.pos_b = n->pos_batch_stride;
   a.eps = n->eps;
-  const float* w[2] = {n->q_weight, n->k_weight};
+  const xfold_heads *x[2] = {&n->q, &n->k}, *y[2] = {&n->q_result, &n->k_result}, *d[2] = {&n->q_grad, &n->k_grad};
   for (int i = 0; i < 2; ++i) {
-    a.t[i].H = i ? n->Hk : n->Hq;
-    a.t[i].w = w[i];
-    a.t[i].scale = i ? 1.f : n->q_scale;
+    QkTensor& t = a.t[i];
+    t.H = i ? n->Hk : n->Hq;
+    t.w = i ? n->k_weight : n->q_weight;
+    t.scale = i ? 1.f : n->q_scale;
+    if (!t.H || !a.B || !a.S) continue;
+    if (!x[i]->at || !y[i]->at || (grad && !d[i]->at)) return fail(c, XFOLD_ERR_ARG, "%s: null argument", what);
+    t.x = x[i]->at; t.xb = x[i]->batch; t.xt = x[i]->token; t.xh = x[i]->head;
+    t.y = const_cast<void*>(y[i]->at); t.yb = y[i]->batch; t.yt = y[i]->token; t.yh = y[i]->head;
+    if (grad) { t.d = d[i]->at; t.db = d[i]->batch; t.dt = d[i]->token; t.dh = d[i]->head; }
+    if (((uintptr_t)t.x | (uintptr_t)t.y | (uintptr_t)t.d) % (n->is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "%s: alignment", what);
   }
   return XFOLD_OK;
 }
-
-static void qk_strides(const long long s[3], long long& b, long long& t, long long& h) { b = s[0]; t = s[1]; h = s[2]; }
 
 }  // namespace xf
 
@@ -857,29 +863,13 @@ int xfold_relative_bias_bwd(xfold_ctx* cx, const void* grad, int is_f32, long lo
   return check_launch(c, "rel_bias_grad_sum_kernel");
 }
 
-int xfold_qk_norm_rotate_fwd(xfold_ctx* cx, const xfold_qk_norm* n, const void* q, const long long q_strides[3], const void* k,
-                             const long long k_strides[3], void* q_out, const long long q_out_strides[3], void* k_out,
-                             const long long k_out_strides[3], void* stream) {
+int xfold_qk_norm_rotate_fwd(xfold_ctx* cx, const xfold_qk_norm* n, void* stream) {
   if (!cx) return XFOLD_ERR_ARG;
   Ctx* c = reinterpret_cast<Ctx*>(cx);
   CallLock call(c);
   QkArgs a;
-  if (int rc = qk_fill(c, n, a, "qk norm")) return rc;
+  if (int rc = qk_fill(c, n, a, false, "qk norm")) return rc;
   if (!a.B || !a.S || !(n->Hq + n->Hk)) return XFOLD_OK;
-  if ((n->Hq && (!q || !q_out || !q_strides || !q_out_strides)) || (n->Hk && (!k || !k_out || !k_strides || !k_out_strides)))
-    return fail(c, XFOLD_ERR_ARG, "qk norm: null argument");
-  const void* x[2] = {q, k};
-  void* y[2] = {q_out, k_out};
-  const long long *xs[2] = {q_strides, k_strides}, *ys[2] = {q_out_strides, k_out_strides};
-  for (int i = 0; i < 2; ++i) {
-    QkTensor& t = a.t[i];
-    if (!t.H) continue;
-    if (((uintptr_t)x[i] | (uintptr_t)y[i]) % (n->is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "qk norm: alignment");
-    t.x = x[i];
-    t.y = y[i];
-    qk_strides(xs[i], t.xb, t.xt, t.xh);
-    qk_strides(ys[i], t.yb, t.yt, t.yh);
-  }
   DeviceGuard dev(c);
   return launch_qk<false>(c, a, n->is_f32, n->neighbours, (cudaStream_t)stream);
 }
@@ -888,37 +878,18 @@ size_t xfold_qk_norm_rotate_bwd_workspace_bytes(xfold_ctx* cx, int D) {
   return cx && D > 0 ? (size_t)qk_ctas(reinterpret_cast<const Ctx*>(cx)) * 2 * D * sizeof(float) : 0;
 }
 
-int xfold_qk_norm_rotate_bwd(xfold_ctx* cx, const xfold_qk_norm* n, const void* dq_out, const long long dq_out_strides[3],
-                             const void* dk_out, const long long dk_out_strides[3], const void* q, const long long q_strides[3],
-                             const void* k, const long long k_strides[3], void* dq, const long long dq_strides[3], void* dk,
-                             const long long dk_strides[3], float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes,
-                             void* stream) {
+int xfold_qk_norm_rotate_bwd(xfold_ctx* cx, const xfold_qk_norm* n, float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes, void* stream) {
   if (!cx) return XFOLD_ERR_ARG;
   Ctx* c = reinterpret_cast<Ctx*>(cx);
   CallLock call(c);
   QkArgs a;
-  if (int rc = qk_fill(c, n, a, "qk norm gradient")) return rc;
+  if (int rc = qk_fill(c, n, a, true, "qk norm gradient")) return rc;
   DeviceGuard dev(c);
   cudaStream_t st = (cudaStream_t)stream;
   if (!a.B || !a.S || !(n->Hq + n->Hk)) {
     for (float* w : {dq_weight, dk_weight})
       if (w && cudaMemsetAsync(w, 0, sizeof(float) * a.D, st) != cudaSuccess) return check_launch(c, "qk norm gradient");
     return XFOLD_OK;
-  }
-  const void *x[2] = {q, k}, *d[2] = {dq_out, dk_out};
-  void* y[2] = {dq, dk};
-  const long long *xs[2] = {q_strides, k_strides}, *ds[2] = {dq_out_strides, dk_out_strides}, *ys[2] = {dq_strides, dk_strides};
-  for (int i = 0; i < 2; ++i) {
-    QkTensor& t = a.t[i];
-    if (!t.H) continue;
-    if (!x[i] || !d[i] || !y[i] || !xs[i] || !ds[i] || !ys[i]) return fail(c, XFOLD_ERR_ARG, "qk norm gradient: null argument");
-    if (((uintptr_t)x[i] | (uintptr_t)y[i] | (uintptr_t)d[i]) % (n->is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "qk norm gradient: alignment");
-    t.x = x[i];
-    t.d = d[i];
-    t.y = y[i];
-    qk_strides(xs[i], t.xb, t.xt, t.xh);
-    qk_strides(ds[i], t.db, t.dt, t.dh);
-    qk_strides(ys[i], t.yb, t.yt, t.yh);
   }
   if (!ws || (uintptr_t)ws % 4 || ws_bytes < xfold_qk_norm_rotate_bwd_workspace_bytes(cx, a.D))
     return fail(c, XFOLD_ERR_ARG, "qk norm gradient: workspace too small");

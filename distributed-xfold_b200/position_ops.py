@@ -5,26 +5,29 @@ Like the rest of the package these calls are not part of an autograd graph: the 
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from ._cabi import QkNorm, XfoldError, check, ctx, load
-from .ops import BF16, _dev, _need_cuda, _ptr, _stream, _Workspace
+from ._cabi import QK_NORM, XfoldError, check, ctx, load
+from .ops import BF16, _need_cuda, _ptr, _stream, _Workspace
 
 F32, I32 = torch.float32, torch.int32
 
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise XfoldError(what)
+def _refuse(what: str):
+    raise XfoldError(what)
 
 
-def _gpu(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    _need_cuda(first, *others)
+def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    dev = first.get_device()
     for t in others:
-        _require(t is None or t.device == first.device, "tensors of one call lie on one device")
+        if t is not None and t.get_device() != dev:
+            _need_cuda(first, *others)
+            _refuse("tensors of one call lie on one device")
+    if dev < 0:
+        _need_cuda(first)
+    return dev
 
 
 # ---------------------------------------------------------------------------------------------
@@ -42,7 +45,8 @@ def logarithmic_buckets(num_buckets: int, max_distance: int, both_sides: bool = 
     side = num_buckets // 2 if both_sides else num_buckets
     single = side // 2
     steps = side - single
-    _require(single >= 1 and max_distance > single and not (both_sides and num_buckets % 2), "logarithmic buckets: too few, or odd")
+    if single < 1 or max_distance <= single or (both_sides and num_buckets % 2):
+        _refuse("logarithmic buckets: too few, or odd")
 
     def bucket(n: int) -> int:
         if n < single:
@@ -57,14 +61,22 @@ def logarithmic_buckets(num_buckets: int, max_distance: int, both_sides: bool = 
     return tuple(bucket(max(-d, 0)) for d in range(-max_distance, max_distance + 1))
 
 
-def _check_relative(buckets, q_pos, k_pos, q_group, k_group) -> None:
-    for t, name in ((buckets, "buckets"), (q_pos, "query positions"), (k_pos, "key positions"), (q_group, "query groups"),
-                    (k_group, "key groups")):
-        _require(t is None or (t.dtype == I32 and t.dim() == 1 and t.is_contiguous()), f"relative bias: {name} are an int32 vector")
-    _require(buckets.numel() % 2 == 1, "relative bias: buckets of the offsets -reach .. reach")
-    _require((q_group is None) == (k_group is None), "relative bias: groups of queries and keys come together")
-    if q_group is not None:
-        _require(q_group.shape == q_pos.shape and k_group.shape == k_pos.shape, "relative bias: a group for each position")
+def _vector(t: torch.Tensor, name: str) -> int:
+    if t.dtype is not I32 or (t.stride() != (1,) and (t.dim() != 1 or t.numel() > 1)):
+        _refuse("relative bias: " + name + " are an int32 vector")
+    return t.numel()
+
+
+def _check_relative(buckets, q_pos, k_pos, q_group, k_group) -> Tuple[int, int, int]:
+    """(reach, queries, keys)"""
+    n, sq, sk = _vector(buckets, "buckets"), _vector(q_pos, "query positions"), _vector(k_pos, "key positions")
+    if n % 2 == 0:
+        _refuse("relative bias: buckets of the offsets -reach .. reach")
+    if (q_group is None) is not (k_group is None):
+        _refuse("relative bias: groups of queries and keys come together")
+    if q_group is not None and (_vector(q_group, "query groups") != sq or _vector(k_group, "key groups") != sk):
+        _refuse("relative bias: a group for each position")
+    return n // 2, sq, sk
 
 
 def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_pos: torch.Tensor, k_pos: Optional[torch.Tensor] = None,
@@ -80,17 +92,19 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_pos: to
     its entries not a number."""
     if k_pos is None:
         k_pos, k_group = q_pos, (q_group if k_group is None else k_group)
-    _require(table.dtype == F32 and table.dim() == 2 and table.is_contiguous(), "relative bias: table is float32 [buckets, heads]")
-    _check_relative(buckets, q_pos, k_pos, q_group, k_group)
-    _require(prepared or dtype in (F32, BF16), "relative bias: float32 or bfloat16")
-    _gpu(table, buckets, q_pos, k_pos, q_group, k_group)
-    dev = _dev(table)
-    (nb, h), sq, sk = table.shape, q_pos.numel(), k_pos.numel()
-    shape = (h, sq, (sk + 7) // 8 * 8 if prepared else sk)
-    out = torch.empty(shape, dtype=torch.float16 if prepared else dtype, device=table.device)
-    check(load().xfold_relative_bias_fwd(ctx(dev), _ptr(table), nb, h, _ptr(buckets), buckets.numel() // 2, _ptr(q_pos), _ptr(k_pos),
-                                         _ptr(q_group), _ptr(k_group), sq, sk, 2 if prepared else int(dtype == BF16), _ptr(out),
-                                         _stream(dev)), dev, "xfold_relative_bias_fwd")
+    if table.dtype is not F32 or table.dim() != 2 or not table.is_contiguous():
+        _refuse("relative bias: table is float32 [buckets, heads]")
+    reach, sq, sk = _check_relative(buckets, q_pos, k_pos, q_group, k_group)
+    nb, h = table.shape
+    if prepared:
+        out, form = (h, sq, (sk + 7) // 8 * 8), 2
+    else:
+        out, form = (h, sq, sk), 0 if dtype is F32 else 1 if dtype is BF16 else _refuse("relative bias: float32 or bfloat16")
+    dev = _device(table, buckets, q_pos, k_pos, q_group, k_group)
+    out = table.new_empty(out) if form == 0 else table.new_empty(out, dtype=torch.float16 if prepared else dtype)
+    rc = load().xfold_relative_bias_fwd(ctx(dev), table.data_ptr(), nb, h, buckets.data_ptr(), reach, q_pos.data_ptr(), k_pos.data_ptr(),
+                                        _ptr(q_group), _ptr(k_group), sq, sk, form, out.data_ptr(), _stream(dev))
+    check(rc, dev, "xfold_relative_bias_fwd")
     return out
 
 
@@ -102,20 +116,24 @@ def relative_position_bias_backward(grad: torch.Tensor, num_buckets: int, bucket
     broadcast).  Sums in 32 bits, in a fixed order."""
     if k_pos is None:
         k_pos, k_group = q_pos, (q_group if k_group is None else k_group)
-    _check_relative(buckets, q_pos, k_pos, q_group, k_group)
-    _require(grad.dtype in (F32, BF16) and grad.dim() == 3, "relative bias gradient: float32 or bfloat16 [heads, queries, keys]")
-    h, sq, sk = grad.shape
-    _require(sq == q_pos.numel() and sk == k_pos.numel(), "relative bias gradient: a position for each query and key")
-    _gpu(grad, buckets, q_pos, k_pos, q_group, k_group)
+    reach, sq, sk = _check_relative(buckets, q_pos, k_pos, q_group, k_group)
+    f32 = grad.dtype is F32
+    if not (f32 or grad.dtype is BF16) or grad.dim() != 3:
+        _refuse("relative bias gradient: float32 or bfloat16 [heads, queries, keys]")
+    h = grad.shape[0]
+    if grad.shape[1] != sq or grad.shape[2] != sk:
+        _refuse("relative bias gradient: a position for each query and key")
+    dev = _device(grad, buckets, q_pos, k_pos, q_group, k_group)
     if sk > 1 and grad.stride(2) != 1:
         grad = grad.contiguous()
-    dev = _dev(grad)
-    lib = load()
-    dtable = torch.empty(num_buckets, h, dtype=F32, device=grad.device)
-    ws = _Workspace.get(dev, max(lib.xfold_relative_bias_bwd_workspace_bytes(ctx(dev), num_buckets, h, sq, sk), 16))
-    check(lib.xfold_relative_bias_bwd(ctx(dev), _ptr(grad), int(grad.dtype == F32), grad.stride(0), grad.stride(1), num_buckets, h,
-                                      _ptr(buckets), buckets.numel() // 2, _ptr(q_pos), _ptr(k_pos), _ptr(q_group), _ptr(k_group),
-                                      sq, sk, _ptr(dtable), _ptr(ws), ws.numel(), _stream(dev)), dev, "xfold_relative_bias_bwd")
+    sh, sr, _ = grad.stride()
+    lib, c = load(), ctx(dev)
+    dtable = q_pos.new_empty((num_buckets, h), dtype=F32)
+    ws = _Workspace.get(dev, lib.xfold_relative_bias_bwd_workspace_bytes(c, num_buckets, h, sq, sk) or 16)
+    rc = lib.xfold_relative_bias_bwd(c, grad.data_ptr(), f32, sh, sr, num_buckets, h, buckets.data_ptr(), reach, q_pos.data_ptr(),
+                                     k_pos.data_ptr(), _ptr(q_group), _ptr(k_group), sq, sk, dtable.data_ptr(), ws.data_ptr(), ws.numel(),
+                                     _stream(dev))
+    check(rc, dev, "xfold_relative_bias_bwd")
     return dtable
 
 
@@ -134,44 +152,61 @@ class Rotation(NamedTuple):
         return cls(float(base) ** (-torch.arange(half, dtype=torch.float64) / max(half, 1)).to(device), interleaved)
 
 
-_Strides = C.c_longlong * 3
-
-
-def _strides(t: torch.Tensor) -> "C.Array":
+def _heads(t: torch.Tensor, name: str) -> Tuple[int, int, int, int]:
+    """(address, strides of batch, tokens and heads)"""
     s = t.stride()
-    return _Strides(s[0], s[1], s[2]) if len(s) == 4 else _Strides(0, s[0], s[1])
+    if len(s) == 4:
+        b, n, h, e = s
+    elif len(s) == 3:
+        (n, h, e), b = s, 0
+    else:
+        _refuse(name + ": bfloat16 or float32 [tokens, heads, width] or [batch, tokens, heads, width]")
+    if e != 1 and t.shape[-1] > 1:
+        _refuse(name + ": a head's elements lie next to each other")
+    return t.data_ptr(), b, n, h
 
 
-def _heads(t: torch.Tensor, like: Optional[torch.Tensor], name: str) -> None:
-    _require(t.dim() in (3, 4) and t.dtype in (BF16, F32), f"{name}: bfloat16 or float32 [tokens, heads, width] or [batch, tokens, heads, width]")
-    _require(t.stride(-1) == 1 or t.shape[-1] == 1, f"{name}: a head's elements lie next to each other")
-    if like is not None:
-        _require(t.shape == like.shape and t.dtype == like.dtype, f"{name}: of the same shape and type as its input")
-
-
-def _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale) -> QkNorm:
-    _heads(q, None, "queries")
-    _heads(k, None, "keys")
-    _require(q.dim() == k.dim() and q.dtype == k.dtype and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1],
-             "queries and keys: the same tokens, width and type")
-    b, s = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
-    d = q.shape[-1]
-    for w in (q_weight, k_weight):
-        _require(w is None or (w.dtype == F32 and tuple(w.shape) == (d,) and w.is_contiguous()), "norm weights: float32 [width]")
-    rot, pos_b = 0, 0
+def _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale):
+    """(device, the call's description up to q and k)"""
+    at_q, at_k = _heads(q, "queries"), _heads(k, "keys")
+    shape, of_k, dt = q.shape, k.shape, q.dtype
+    if dt is not BF16 and dt is not F32:
+        _refuse("queries and keys: bfloat16 or float32 [tokens, heads, width] or [batch, tokens, heads, width]")
+    if len(shape) == 3:
+        shape, of_k = (1, *shape), (1, *of_k)
+    b, s, hq, d = shape
+    hk = of_k[-2]
+    if of_k != (b, s, hk, d) or k.dtype is not dt or q.dim() != k.dim():
+        _refuse("queries and keys: the same tokens, width and type")
+    dev = q.get_device()
+    same = k.get_device() == dev
+    qw = kw = rot = inter = freqs = pos = pos_b = 0
+    if q_weight is not None:
+        qw, same = _weight(q_weight, d), same and q_weight.get_device() == dev
+    if k_weight is not None:
+        kw, same = _weight(k_weight, d), same and k_weight.get_device() == dev
     if rotation is not None:
-        f = rotation.freqs
-        _require(f.dtype == torch.float64 and f.dim() == 1 and f.is_contiguous() and 2 * f.numel() <= d,
-                 "rotation: float64 frequencies for pairs of a head's elements")
+        f, inter = rotation
         rot = 2 * f.numel()
+        if f.dtype is not torch.float64 or f.dim() != 1 or rot > d or (f.stride(0) != 1 and rot > 2):
+            _refuse("rotation: float64 frequencies for pairs of a head's elements")
+        freqs, same = f.data_ptr(), same and f.get_device() == dev
     if positions is not None:
-        _require(positions.dtype == I32 and tuple(positions.shape) in ((s,), (b, s)), "positions: int32 [tokens] or [batch, tokens]")
-        _require(positions.stride(-1) == 1 or s <= 1, "positions: a sequence's lie next to each other")
-        pos_b = positions.stride(0) if positions.dim() == 2 else 0
-    _gpu(q, k, q_weight, k_weight, positions, None if rotation is None else rotation.freqs)
-    return QkNorm(b, s, q.shape[-2], k.shape[-2], d, rot, int(rotation is not None and rotation.interleaved), int(q.dtype == F32),
-                  _ptr(q_weight), _ptr(k_weight), None if rotation is None or not rot else _ptr(rotation.freqs), _ptr(positions), pos_b,
-                  eps, q_scale)
+        step = positions.stride()
+        if positions.dtype is not I32 or positions.shape != ((s,) if len(step) == 1 else (b, s)):
+            _refuse("positions: int32 [tokens] or [batch, tokens]")
+        if step[-1] != 1 and s > 1:
+            _refuse("positions: a sequence's lie next to each other")
+        pos, pos_b, same = positions.data_ptr(), step[0] if len(step) == 2 else 0, same and positions.get_device() == dev
+    if dev < 0 or not same:
+        _device(q, k, q_weight, k_weight, positions, None if rotation is None else f)
+    return dev, (b, s, hq, hk, d, rot, bool(inter), dt is F32, qw, kw, freqs, pos, pos_b, eps, q_scale, *at_q, *at_k)
+
+
+def _weight(w: torch.Tensor, d: int) -> int:
+    if w.dtype is not F32 or w.shape != (d,) or (w.stride(0) != 1 and d > 1):
+        _refuse("norm weights: float32 [width]")
+    return w.data_ptr()
 
 
 def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
@@ -181,16 +216,17 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     the rotation by position, in one pass.  q and k: bfloat16 or float32 [batch, tokens, heads, width] or without the batch, widths
     even up to 256, with as many heads each as they like and any strides between them (views of a fused projection).  positions
     int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, which may be the inputs."""
-    n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
+    dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    qo, ko = out
-    _heads(qo, q, "result of the queries")
-    _heads(ko, k, "result of the keys")
-    _gpu(q, qo, ko)
-    dev = _dev(q)
-    check(load().xfold_qk_norm_rotate_fwd(ctx(dev), C.byref(n), _ptr(q), _strides(q), _ptr(k), _strides(k), _ptr(qo), _strides(qo),
-                                          _ptr(ko), _strides(ko), _stream(dev)), dev, "xfold_qk_norm_rotate_fwd")
+        qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+    else:
+        qo, ko = out
+        for o, x in ((qo, q), (ko, k)):
+            if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
+                _refuse("results of queries and keys: shape, type and device of their inputs")
+    rc = load().xfold_qk_norm_rotate_fwd(ctx(dev), QK_NORM.pack(*n, *_heads(qo, "result of the queries"), *_heads(ko, "result of the keys"),
+                                                                0, 0, 0, 0, 0, 0, 0, 0), _stream(dev))
+    check(rc, dev, "xfold_qk_norm_rotate_fwd")
     return qo, ko
 
 
@@ -204,20 +240,19 @@ def norm_rotate_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
                             positions: Optional[torch.Tensor] = None, *, eps: float = 1e-6, q_scale: float = 1.0):
     """(dq, dk, dq_weight, dk_weight) of ``norm_rotate_qk`` from the gradients of its results; q and k are its inputs (kept, where
     the forward ran in place).  The weights' gradients are float32, summed in a fixed order; None for a weight that is None."""
-    n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
-    _gpu(q, dq_out, dk_out)
-    _require(dq_out.shape == q.shape and dq_out.dtype == q.dtype and dk_out.shape == k.shape and dk_out.dtype == k.dtype,
-             "gradients of the results: of the same shape and type as queries and keys")
+    dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
+    for g, x in ((dq_out, q), (dk_out, k)):
+        if g.shape != x.shape or g.dtype is not x.dtype or g.get_device() != dev:
+            _refuse("gradients of the results: shape, type and device of queries and keys")
     if dq_out.stride(-1) != 1:   # (a gradient that was broadcast along the head)
         dq_out = dq_out.contiguous()
     if dk_out.stride(-1) != 1:
         dk_out = dk_out.contiguous()
-    dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-    dev = _dev(q)
-    lib = load()
-    ws = _Workspace.get(dev, lib.xfold_qk_norm_rotate_bwd_workspace_bytes(ctx(dev), n.D))
-    check(lib.xfold_qk_norm_rotate_bwd(ctx(dev), C.byref(n), _ptr(dq_out), _strides(dq_out), _ptr(dk_out), _strides(dk_out), _ptr(q),
-                                       _strides(q), _ptr(k), _strides(k), _ptr(dq), _strides(dq), _ptr(dk), _strides(dk), _ptr(dqw),
-                                       _ptr(dkw), _ptr(ws), ws.numel(), _stream(dev)), dev, "xfold_qk_norm_rotate_bwd")
+    lib, c = load(), ctx(dev)
+    ws = _Workspace.get(dev, lib.xfold_qk_norm_rotate_bwd_workspace_bytes(c, n[4]))
+    desc = QK_NORM.pack(*n, *_heads(dq, ""), *_heads(dk, ""), *_heads(dq_out, ""), *_heads(dk_out, ""))
+    rc = lib.xfold_qk_norm_rotate_bwd(c, desc, _ptr(dqw), _ptr(dkw), ws.data_ptr(), ws.numel(), _stream(dev))
+    check(rc, dev, "xfold_qk_norm_rotate_bwd")
     return dq, dk, dqw, dkw

@@ -275,23 +275,25 @@ int xfold_relative_bias_bwd(xfold_ctx* ctx, const void* grad, int is_f32, long l
  * fused projection; results may lie over their inputs.  weights float32 [D] or NULL (ones); freqs float64 [rot / 2] on the
  * device; positions int32, that of token s of batch entry b at b * pos_batch_stride + s, or NULL (s).  bf16 or float32. */
 typedef struct {
+  const void* at; /* (results are written) */
+  long long batch, token, head; /* strides */
+} xfold_heads;
+typedef struct {
   int B, S, Hq, Hk, D, rot, neighbours, is_f32;
   const float *q_weight, *k_weight;
   const double* freqs;
   const int* positions;
   long long pos_batch_stride;
   float eps, q_scale;
+  xfold_heads q, k;
+  xfold_heads q_result, k_result; /* forward: the results; backward: the gradients of q and k */
+  xfold_heads q_grad, k_grad;     /* backward: the gradients of the forward's results, which its own may lie over */
 } xfold_qk_norm;
-int xfold_qk_norm_rotate_fwd(xfold_ctx* ctx, const xfold_qk_norm* n, const void* q, const long long q_strides[3], const void* k,
-                             const long long k_strides[3], void* q_out, const long long q_out_strides[3], void* k_out,
-                             const long long k_out_strides[3], void* stream);
-/* dq, dk (over the gradients of the results, dq_out and dk_out, if wished) and the weights' gradients, float32 [D], summed in a
- * fixed order (NULL: not wanted); q and k are the forward's inputs. */
+int xfold_qk_norm_rotate_fwd(xfold_ctx* ctx, const xfold_qk_norm* n, void* stream);
+/* The gradients of q and k, and those of the weights, float32 [D], summed in a fixed order (NULL: not wanted); q and k are the
+ * forward's inputs. */
 size_t xfold_qk_norm_rotate_bwd_workspace_bytes(xfold_ctx* ctx, int D);
-int xfold_qk_norm_rotate_bwd(xfold_ctx* ctx, const xfold_qk_norm* n, const void* dq_out, const long long dq_out_strides[3],
-                             const void* dk_out, const long long dk_out_strides[3], const void* q, const long long q_strides[3],
-                             const void* k, const long long k_strides[3], void* dq, const long long dq_strides[3], void* dk,
-                             const long long dk_strides[3], float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes,
+int xfold_qk_norm_rotate_bwd(xfold_ctx* ctx, const xfold_qk_norm* n, float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes,
                              void* stream);
 
 /* ---- linear layers in 8-bit integers (no counterpart in the reference) --------------------------------

@@ -115,7 +115,7 @@ def test_refused_qk(P, kw, what):
     from distributed_xfold_b200._cabi import XfoldError
     if "freqs" in kw:
         kw["rotation"] = P.Rotation(kw.pop("freqs"))
-    with pytest.raises(XfoldError, match=what if "out" not in kw else "GPU only|" + what):
+    with pytest.raises(XfoldError, match=what if "out" not in kw else "GPU only"):
         P.norm_rotate_qk(**_qk(**kw))
 
 
