@@ -33,12 +33,15 @@ struct RelShared {  // what both directions read of the positions
 };
 
 // a lut entry that names no row of the table: row nb + 1
-__device__ __forceinline__ void stage_lut(const RelShared& s, uint16_t* lut) {
+__device__ __forceinline__ void stage_lut(const RelShared& s, uint16_t* lut, int step = 1) {
   for (int i = threadIdx.x; i < 2 * s.reach + 1; i += blockDim.x) {
     const int b = s.lut[i];
-    lut[i] = uint16_t(b >= 0 && b < s.nb ? b : s.nb + 1);
+    lut[i] = uint16_t((b >= 0 && b < s.nb ? b : s.nb + 1) * step);
   }
 }
+// the positions that a query's buckets end at: a key's place in the lut is min(max(its position, low), high) - (query's - reach)
+__device__ __forceinline__ int low_end(int qp, int reach) { return max(qp, -0x7fffffff - 1 + reach) - reach; }
+__device__ __forceinline__ int high_end(int qp, int reach) { return min(qp, 0x7fffffff - reach) + reach; }
 
 struct RelFwdArgs {
   RelShared s;
@@ -143,115 +146,185 @@ static void launch_rel_fwd(Ctx* c, RelFwdArgs a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // Gradient of the table: dtable[b][h] = sum over (i, j) with b(i, j) = b of grad[h][i][j].
 //
-// A lane keeps V columns of one head, goes down the rows and adds to sums of its own: [nb + 2][32 lanes] for each warp in
-// shared memory (a lane's bank is its own: no conflicts, no atomics, and the order of the sum is always the same).  Where the
-// V columns share a bucket their sum stays in a register until the bucket changes.  CTAs leave their sums in the workspace;
-// a second kernel adds them.
+// A warp keeps 32 V columns of one head, V neighbours to a lane, and goes down its rows.  Of each 32 columns (a group of
+// lanes) a row's entries lie before the reach, behind it or in another group of tokens, all of them: then a lane adds its V to
+// one of three sums in registers, at two dozen instructions for 512 bytes.  Or they do not: a band along the diagonal.  Its
+// rows are put into shared memory and taken a column to a lane, into sums [nb + 2][32 lanes] of the warp's (a lane's bank is its
+// own: no conflicts, no atomics, and the order of the sum is always the same).
+// The rows of a CTA lie `slices` apart, so that every warp has its share of the band.  CTAs leave their sums in the workspace; a
+// second kernel adds them.
 // ---------------------------------------------------------------------------------------------
 struct RelBwdArgs {
   RelShared s;
   const void* grad;
-  long long sh, sq;   // strides of heads and queries, in elements
-  float* partial;     // [H][ctas][nb]
-  int cblocks, ctas;  // blocks of columns; CTAs for each head
+  long long sh, sq;       // strides of heads and queries, in elements
+  float* partial;         // [H][slices][nb]
+  int slices;             // CTAs for each head: rows slice, slice + slices, ...
+  int cblocks, row_sets;  // blocks of 32 V columns; sets of rows that warps take such a block in
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
 
-template <typename E, int V, bool VEC>
-__global__ void __launch_bounds__(256) rel_bias_grad_kernel(const RelBwdArgs a) {
-  extern __shared__ uint8_t smem_raw[];
+constexpr int REL_ROWS = 8, REL_HALF = 4;  // rows of a warp that are on their way together; that lie in shared memory
+template <int V>
+__host__ __device__ constexpr size_t rel_bwd_warp_bytes() { return REL_HALF * 512 + 32 * V * 8; }  // rows; columns' positions, groups
+
+// sum of a piece
+__device__ __forceinline__ float piece_sum(const RelPiece<float, 4>& p) { return (p.e[0] + p.e[1]) + (p.e[2] + p.e[3]); }
+__device__ __forceinline__ float piece_sum(const RelPiece<bf16, 8>& p) {
+  const uint4 u = *reinterpret_cast<const uint4*>(&p);
+  float2 t = make_float2(bf16_lo(u.x), bf16_hi(u.x));
+  sum2(u.y, t);
+  sum2(u.z, t);
+  sum2(u.w, t);
+  return t.x + t.y;
+}
+
+template <typename E, int V, bool VEC, bool GROUPS>
+__global__ void __launch_bounds__(256, VEC ? 3 : 2) rel_bias_grad_kernel(const RelBwdArgs a) {
+  static_assert(sizeof(E) * V == 16, "a row's 32 V columns take 512 bytes");
+  constexpr int W = 32 * V, SHARE = 32 / V;  // columns of a warp; lanes whose neighbours make 32 columns
+  extern __shared__ __align__(16) uint8_t smem_raw[];
   const RelShared& s = a.s;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hrows = s.nb + 2;
-  float* sums = reinterpret_cast<float*>(smem_raw);
+  uint8_t* own = smem_raw + warp * rel_bwd_warp_bytes<V>();
+  E* srow = reinterpret_cast<E*>(own);  // [REL_HALF][W]
+  int* skp = reinterpret_cast<int*>(own + REL_HALF * 512);
+  int* skg = skp + W;
+  float* sums = reinterpret_cast<float*>(smem_raw + warps * rel_bwd_warp_bytes<V>());
   uint16_t* lut = reinterpret_cast<uint16_t*>(sums + (size_t)warps * hrows * 32);
   float* acc = sums + (size_t)warp * hrows * 32 + lane;
   pdl_wait();
   pdl_launch();
-  stage_lut(s, lut);
-  for (int b = 0; b < hrows; ++b) acc[b * 32] = 0.f;
-  __syncthreads();
-  const int h = blockIdx.x / a.ctas, cta = blockIdx.x % a.ctas, cb = cta % a.cblocks, rg = cta / a.cblocks, rgs = a.ctas / a.cblocks;
-  // VEC: V neighbours; else every 32nd column, so that a warp's loads lie together
-  const int c0 = cb * 32 * V, step = VEC ? 1 : 32, first = c0 + (VEC ? lane * V : lane);
-  int kp[V], kg[V], pmin = 0x7fffffff, pmax = -0x7fffffff - 1, nv = 0;
-  bool whole = true;
+  const int h = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+  const int rows = (s.Sq - slice + a.slices - 1) / a.slices;  // of this CTA
+  const E* g0 = static_cast<const E*>(a.grad) + (long long)h * a.sh;
+  float before = 0.f, behind = 0.f, others = 0.f;
+  bool staged = false;  // (the table of buckets and the sums are made while the first unit's rows are on their way)
+  auto stage = [&]() {
+    stage_lut(s, lut, 32);  // (at most 1025 * 32)
+    for (int b = 0; b < hrows; ++b) acc[b * 32] = 0.f;
+    named_bar_sync(1, blockDim.x);
+    staged = true;
+  };
+  for (int unit = warp; unit < a.cblocks * a.row_sets; unit += warps) {
+    const int c0 = unit % a.cblocks * W, set = unit / a.cblocks, c1 = c0 + lane * V;
+    RelPiece<E, V> x[REL_ROWS];
+    int qp = 0, qg = 0;  // lane u: of row u of the batch
+    const E* next = g0 + ((long long)set * a.slices + slice) * a.sq + (VEC && c1 < s.Sk ? c1 : 0);
+    const long long step = (long long)a.row_sets * a.slices * a.sq;
+    auto load = [&](int n0) {  // rows n0, n0 + row_sets, ..; rows and columns beyond the last are read as the last, and not added
+      const int last = (rows - 1 - n0) / a.row_sets;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int j = first + v * step;
-    const bool in = j < s.Sk;
-    kp[v] = in ? s.k_pos[j] : 0;
-    kg[v] = in && s.k_grp ? s.k_grp[j] : 0;
-    if (in) {
-      ++nv;
-      whole = whole && kg[v] == kg[0];
-      pmin = min(pmin, kp[v]);
-      pmax = max(pmax, kp[v]);
-    }
-  }
-  const E* g = static_cast<const E*>(a.grad) + (long long)h * a.sh + first;
-  constexpr int U = 4;
-  int cur = s.nb;  // the bucket whose sum is in `run`
-  float run = 0.f;
-  const int stride = rgs * warps;
-  if (nv > 0) {
-    for (int i0 = rg * warps + warp; i0 < s.Sq; i0 += stride * U) {
-      float x[U][V];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * stride;
-        const E* row = g + (long long)i * a.sq;
-        if (VEC && nv == V && i < s.Sq) {
-          const RelPiece<E, V> p = *reinterpret_cast<const RelPiece<E, V>*>(row);
-#pragma unroll
-          for (int v = 0; v < V; ++v) x[u][v] = to_float(p.e[v]);
+      for (int u = 0; u < REL_ROWS; ++u) {
+        const E* row = next + min(u, last) * step;
+        if constexpr (VEC) {
+          x[u] = *reinterpret_cast<const RelPiece<E, V>*>(row);
         } else {
 #pragma unroll
-          for (int v = 0; v < V; ++v) x[u][v] = i < s.Sq && first + v * step < s.Sk ? to_float(row[v * step]) : 0.f;
+          for (int v = 0; v < V; ++v) x[u].e[v] = row[min(c0 + v * 32 + lane, s.Sk - 1)];
         }
       }
+      next += REL_ROWS * step;
+      const int i = min(n0 + (lane & (REL_ROWS - 1)) * a.row_sets, rows - 1) * a.slices + slice;
+      qp = s.q_pos[i];
+      if (GROUPS) qg = s.q_grp[i];
+    };
+    if (set < rows) load(set);
+    __syncwarp();
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * stride;
-        if (i >= s.Sq) break;
-        const int qp = s.q_pos[i], qg = s.q_grp ? s.q_grp[i] : 0;
-        const int lo = offset_in_lut(pmin, qp, s.reach), hi = offset_in_lut(pmax, qp, s.reach);
-        const bool other = whole && kg[0] != qg;
-        if (other || (whole && lo == hi)) {
-          const int b = other ? s.nb - 1 : int(lut[lo]);
-          float t = x[u][0];
+    for (int v = 0; v < V; ++v) {
+      const int j = min(c0 + v * 32 + lane, s.Sk - 1);
+      skp[v * 32 + lane] = s.k_pos[j];
+      if (GROUPS) skg[v * 32 + lane] = s.k_grp[j];
+    }
+    if (!staged) stage();
+    __syncwarp();
+    // the lane's 32 columns: before the reach of rows at `after` or later, behind that of rows at `until` or earlier
+    int lo = skp[lane * V], hi = lo, grp = GROUPS ? skg[lane * V] : 0, gmax = grp;  // (columns beyond the last repeat it)
 #pragma unroll
-          for (int v = 1; v < V; ++v) t += x[u][v];
-          if (b != cur) {
-            acc[cur * 32] += run;
-            cur = b;
-            run = 0.f;
-          }
-          run += t;
-        } else {
+    for (int v = 1; v < V; ++v) {
+      lo = min(lo, skp[lane * V + v]); hi = max(hi, skp[lane * V + v]);
+      if (GROUPS) { grp = min(grp, skg[lane * V + v]); gmax = max(gmax, skg[lane * V + v]); }
+    }
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            if (first + v * step >= s.Sk) break;
-            const int b = kg[v] != qg ? s.nb - 1 : int(lut[offset_in_lut(kp[v], qp, s.reach)]);
-            if (b != cur) {
-              acc[cur * 32] += run;
-              cur = b;
-              run = 0.f;
+    for (int o = 1; o < SHARE; o <<= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o)); hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      if (GROUPS) { grp = min(grp, __shfl_xor_sync(0xffffffffu, grp, o)); gmax = max(gmax, __shfl_xor_sync(0xffffffffu, gmax, o)); }
+    }
+    const bool fits = hi <= 0x7fffffff - s.reach && lo >= s.reach - 0x7fffffff;  // (else as a band)
+    const int after = fits ? hi + s.reach : 0, until = fits ? lo - s.reach : 0;
+    const bool mine = c1 < s.Sk, same = grp == gmax && fits;
+    for (int n0 = set; n0 < rows; n0 += REL_ROWS * a.row_sets) {
+      const int bp = qp, bg = qg;
+#pragma unroll
+      for (int half = 0; half < REL_ROWS; half += REL_HALF) {
+        uint32_t band = 0;  // lane u: the lanes of row u whose columns lie in the band
+#pragma unroll
+        for (int u = half; u < half + REL_HALF; ++u) {
+          if (n0 + u * a.row_sets < rows) {
+            const int p = __shfl_sync(0xffffffffu, bp, u), g = GROUPS ? __shfl_sync(0xffffffffu, bg, u) : 0;
+            const bool other = GROUPS && same && grp != g, in = same && (!GROUPS || grp == g), bef = in && after <= p, beh = in && until >= p;
+            const bool out = other || bef || beh;
+            const uint32_t b = __ballot_sync(0xffffffffu, mine && !out);
+            E* row = srow + (u - half) * W;
+            if constexpr (!VEC) {  // a lane's columns lie apart: everything passes through shared memory
+#pragma unroll
+              for (int v = 0; v < V; ++v) row[v * 32 + lane] = x[u].e[v];
+              __syncwarp();
+              x[u] = *reinterpret_cast<const RelPiece<E, V>*>(row + lane * V);
+#pragma unroll
+              for (int v = 0; v < V; ++v)
+                if (c1 + v >= s.Sk) x[u].e[v] = E(0.f);
+            } else if (b) {
+              *reinterpret_cast<RelPiece<E, V>*>(row + lane * V) = x[u];
             }
-            run += x[u][v];
+            const float t = mine ? piece_sum(x[u]) : 0.f;
+            if (beh) behind += t;  // (with a reach of nothing a key at the query's own position is on both sides)
+            else if (bef) before += t;
+            if (GROUPS && other) others += t;
+            if (lane == u) band = b;
           }
         }
+        __syncwarp();
+        if (half + REL_HALF == REL_ROWS && n0 + REL_ROWS * a.row_sets < rows) load(n0 + REL_ROWS * a.row_sets);
+        uint32_t todo = __ballot_sync(0xffffffffu, band != 0);
+        while (todo) {
+          const int u = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const int p = __shfl_sync(0xffffffffu, bp, u), g = GROUPS ? __shfl_sync(0xffffffffu, bg, u) : 0;
+          const int low = low_end(p, s.reach), high = high_end(p, s.reach);
+          const E* row = srow + (u - half) * W + lane;
+          uint32_t b = __shfl_sync(0xffffffffu, band, u);
+          do {
+            const int at = (__ffs(b) - 1) / SHARE * 32;  // the first 32 columns left
+            b &= ~(((1u << SHARE) - 1) << (at / 32 * SHARE));
+            int k = lut[min(max(skp[at + lane], low), high) - p + s.reach];
+            if (GROUPS && skg[at + lane] != g) k = (s.nb - 1) * 32;
+            if (c0 + at + lane < s.Sk) acc[k] += to_float(row[at]);
+          } while (b);
+        }
+        __syncwarp();
       }
     }
-    acc[cur * 32] += run;
   }
+  if (!staged) stage();
+  acc[lut[0]] += before;
+  acc[lut[2 * s.reach]] += behind;
+  acc[(s.nb - 1) * 32] += others;
   __syncthreads();
-  for (int b = warp; b < s.nb; b += warps) {
+  // four threads for a bucket, eight lanes' sums of every warp to each
+  for (int b = threadIdx.x >> 2; b < (s.nb + 7) / 8 * 8; b += blockDim.x >> 2) {
     float t = 0.f;
-    for (int w = 0; w < warps; ++w) t += sums[((size_t)w * hrows + b) * 32 + lane];
-    t = warp_total(t);
-    if (lane == 0) a.partial[((long long)h * a.ctas + cta) * s.nb + b] = t;
+    if (b < s.nb)
+      for (int w = 0; w < warps; ++w) {
+        const float4* q = reinterpret_cast<const float4*>(sums + ((size_t)w * hrows + b) * 32) + (threadIdx.x & 3) * 2;
+        t += ((q[0].x + q[0].y) + (q[0].z + q[0].w)) + ((q[1].x + q[1].y) + (q[1].z + q[1].w));
+      }
+    t += __shfl_xor_sync(0xffffffffu, t, 1);
+    t += __shfl_xor_sync(0xffffffffu, t, 2);
+    if (b < s.nb && (threadIdx.x & 3) == 0) a.partial[((long long)h * a.slices + slice) * s.nb + b] = t;
   }
 }
 
@@ -269,33 +342,48 @@ __global__ void __launch_bounds__(256) rel_bias_grad_sum_kernel(const float* par
 }
 
 struct RelBwdPlan {
-  int warps, cblocks, ctas;
+  int warps, slices, cblocks, row_sets;
   size_t smem;
 };
-static RelBwdPlan rel_bwd_plan(int nb, int H, int Sq, int Sk, int reach, int V, int sms) {
+// CTAs for each head: three or two to an SM, by their registers and their sums' room
+static int rel_bwd_slices(int nb, int H, int Sq, bool vec, int sms) {
+  const int per_sm = vec && (size_t)(nb + 2) * 128 * 8 <= 36 * 1024 ? 3 : 2;
+  return std::max(1, std::min(per_sm * sms / H, (Sq + 7) / 8));
+}
+static RelBwdPlan rel_bwd_plan(int nb, int H, int Sq, int Sk, int reach, int V, bool vec, int sms) {
   RelBwdPlan p;
-  const size_t per_warp = (size_t)(nb + 2) * 128;
+  const size_t per_warp = (size_t)(nb + 2) * 128 + (V == 8 ? rel_bwd_warp_bytes<8>() : rel_bwd_warp_bytes<4>()), rest = (2 * reach + 1) * 2;
   p.warps = 8;
-  while (p.warps > 1 && p.warps * per_warp > 100 * 1024) p.warps /= 2;
-  p.smem = p.warps * per_warp + (2 * reach + 1) * 2;
+  while (p.warps > 1 && p.warps * per_warp + rest > 113 * 1024) p.warps /= 2;
+  p.smem = p.warps * per_warp + rest;
+  p.slices = rel_bwd_slices(nb, H, Sq, vec, sms);
   p.cblocks = (Sk + 32 * V - 1) / (32 * V);
-  const long long resident = 2ll * sms, slices = std::max(1ll, resident / std::max(1ll, (long long)H * p.cblocks));
-  const long long most = std::max(1, (Sq + p.warps * 4 - 1) / (p.warps * 4));
-  p.ctas = (int)(p.cblocks * std::min(slices, most));
+  // sets of rows: the warps' rounds over the units are to come out even, but a unit costs about as much as four rows to begin
+  const int rows = (Sq + p.slices - 1) / p.slices;
+  double best = 1e30;
+  for (int n = 1; n <= 8; n *= 2) {
+    const double cost = double((p.cblocks * n + p.warps - 1) / p.warps) * ((rows + n - 1) / n + 4);
+    if (cost < best) {
+      best = cost;
+      p.row_sets = n;
+    }
+  }
   return p;
 }
 
 template <typename E, int V, bool VEC>
 static int launch_rel_bwd(Ctx* c, RelBwdArgs a, const RelBwdPlan& p, cudaStream_t st) {
-  auto kern = rel_bias_grad_kernel<E, V, VEC>;
+  auto kern = a.s.k_grp ? rel_bias_grad_kernel<E, V, VEC, true> : rel_bias_grad_kernel<E, V, VEC, false>;
   static bool attr_done[8] = {false};
   if (!attr_done[c->device & 7]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    cudaError_t e = cudaFuncSetAttribute(rel_bias_grad_kernel<E, V, VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(rel_bias_grad_kernel<E, V, VEC, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e != cudaSuccess) return fail(c, XFOLD_ERR_LAUNCH, "relative bias gradient: %s", cudaGetErrorString(e));
     attr_done[c->device & 7] = true;
   }
   ProfScope ps(c, XFOLD_K_MASK_BIAS, st);
-  launch_pdl(kern, dim3(a.s.H * a.ctas), p.warps * 32, p.smem, st, a);
+  launch_pdl(kern, dim3(a.s.H * a.slices), p.warps * 32, p.smem, st, a);
   return check_launch(c, "rel_bias_grad_kernel");
 }
 
@@ -819,10 +907,7 @@ int xfold_relative_bias_fwd(xfold_ctx* cx, const float* table, int num_buckets, 
 size_t xfold_relative_bias_bwd_workspace_bytes(xfold_ctx* cx, int num_buckets, int H, int Sq, int Sk) {
   if (!cx || num_buckets < 1 || H < 1 || Sq < 1 || Sk < 1) return 0;
   const Ctx* c = reinterpret_cast<const Ctx*>(cx);
-  size_t most = 0;
-  for (int V : {4, 8})  // what the call takes goes by type and alignment
-    most = std::max(most, (size_t)rel_bwd_plan(num_buckets, H, Sq, Sk, 0, V, c->sm_count).ctas);
-  return most * H * num_buckets * sizeof(float);
+  return (size_t)rel_bwd_slices(num_buckets, H, Sq, true, c->sm_count) * H * num_buckets * sizeof(float);
 }
 
 int xfold_relative_bias_bwd(xfold_ctx* cx, const void* grad, int is_f32, long long head_stride, long long query_stride, int num_buckets,
@@ -842,9 +927,9 @@ int xfold_relative_bias_bwd(xfold_ctx* cx, const void* grad, int is_f32, long lo
   }
   if (!grad || (uintptr_t)grad % (is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "relative bias gradient: the gradient's address");
   const int V = is_f32 ? 4 : 8;
-  const RelBwdPlan p = rel_bwd_plan(num_buckets, H, Sq, Sk, reach, V, c->sm_count);
-  if ((long long)H * p.ctas > 0x7fffffffll) return fail(c, XFOLD_ERR_ARG, "relative bias gradient: too many heads and keys");
-  if (!ws || (uintptr_t)ws % 4 || ws_bytes < sizeof(float) * (size_t)H * p.ctas * num_buckets)
+  const bool vec = (uintptr_t)grad % 16 == 0 && head_stride % V == 0 && query_stride % V == 0 && Sk % V == 0;
+  const RelBwdPlan p = rel_bwd_plan(num_buckets, H, Sq, Sk, reach, V, vec, c->sm_count);
+  if (!ws || (uintptr_t)ws % 4 || ws_bytes < sizeof(float) * (size_t)H * p.slices * num_buckets)
     return fail(c, XFOLD_ERR_ARG, "relative bias gradient: workspace too small");
   RelBwdArgs a{};
   a.s = RelShared{buckets, q_pos, k_pos, q_group, k_group, reach, num_buckets, H, Sq, Sk};
@@ -852,14 +937,14 @@ int xfold_relative_bias_bwd(xfold_ctx* cx, const void* grad, int is_f32, long lo
   a.sh = head_stride;
   a.sq = query_stride;
   a.partial = (float*)ws;
+  a.slices = p.slices;
   a.cblocks = p.cblocks;
-  a.ctas = p.ctas;
-  const bool vec = (uintptr_t)grad % 16 == 0 && head_stride % V == 0 && query_stride % V == 0;
+  a.row_sets = p.row_sets;
   int rc = is_f32 ? (vec ? launch_rel_bwd<float, 4, true>(c, a, p, st) : launch_rel_bwd<float, 4, false>(c, a, p, st))
                   : (vec ? launch_rel_bwd<bf16, 8, true>(c, a, p, st) : launch_rel_bwd<bf16, 8, false>(c, a, p, st));
   if (rc) return rc;
   ProfScope ps(c, XFOLD_K_MASK_BIAS, st);
-  launch_pdl(rel_bias_grad_sum_kernel, dim3((num_buckets * H + 7) / 8), 256, 0, st, (const float*)a.partial, dtable, num_buckets, H, p.ctas);
+  launch_pdl(rel_bias_grad_sum_kernel, dim3((num_buckets * H + 7) / 8), 256, 0, st, (const float*)a.partial, dtable, num_buckets, H, p.slices);
   return check_launch(c, "rel_bias_grad_sum_kernel");
 }
 
