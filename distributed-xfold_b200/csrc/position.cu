@@ -404,9 +404,10 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
 // Pairs are (i, i + rot / 2), or neighbours (2 i, 2 i + 1).
 //
 // G lanes share a head; a lane holds two pieces of V elements that rotate into each other: of the halves, or 2 V neighbours
-// (beyond `rot`: 2 V neighbours that do not rotate).  Its place in the head is the same for all heads, so weights, cosines and
-// sines stay in registers while a warp goes through its token's heads.  Angles are made once for a token and warp, in turns and
-// in 64 bits until the whole turns are gone: 32 bits would lose far positions.
+// (beyond `rot`: 2 V neighbours that do not rotate).  Its place in the head is the same for all heads of a token, and so an
+// element of the result is own * A + partner * B (and r, the reciprocal root), with A and B made of weights, cosines and sines
+// once for a token: in registers, at three instructions for two elements.  Angles are made once for a token and warp, in turns
+// and in 64 bits until the whole turns are gone: 32 bits would lose far positions.
 // ---------------------------------------------------------------------------------------------
 struct QkTensor {
   const void *x, *d;  // d: gradient of the result (backward)
@@ -414,16 +415,17 @@ struct QkTensor {
   long long xb, xt, xh, db, dt, dh, yb, yt, yh;  // strides of batch, token and head, in elements
   const float* w;
   float scale;
-  int H, passes;
+  int H, passes, wide_w;   // passes: of a token, as many heads each as a warp has groups of lanes; wide_w: the weights lie at a 16-byte boundary
+  int ctas, share, more;   // a warp takes `share` passes, the first `more` one more
 };
 struct QkArgs {
   QkTensor t[2];
   const double* freqs;
   const int* pos;
   long long pos_b;
-  int B, S, D, rot, log_g, parts, per_part;
+  int B, S, D, rot, log_g;
   float eps;
-  float* partial;  // backward: [CTAs][2][D]
+  float* partial;       // backward: [CTAs][D], those of the queries in front
 };
 
 template <int BYTES>
@@ -439,17 +441,28 @@ struct Piece {
   __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(raw)*>(p) = raw; }
   __device__ __forceinline__ void clear() { raw = decltype(raw){}; }
-  __device__ __forceinline__ void get(float (&f)[V]) const {
-    const T* e = reinterpret_cast<const T*>(&raw);
+  __device__ __forceinline__ void get(float* f) const {
+    if constexpr (sizeof(T) == 4 || V == 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) f[v] = to_float(e[v]);
+      for (int v = 0; v < V; ++v) f[v] = to_float(reinterpret_cast<const T*>(&raw)[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v += 2) {
+        const uint32_t u = reinterpret_cast<const uint32_t*>(&raw)[v / 2];
+        f[v] = bf16_lo(u);
+        f[v + 1] = bf16_hi(u);
+      }
+    }
   }
-  __device__ __forceinline__ void set(const float (&f)[V]) {
-    T* e = reinterpret_cast<T*>(&raw);
+  __device__ __forceinline__ void set(const float* f) {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if constexpr (sizeof(T) == 4) e[v] = f[v];
-      else e[v] = __float2bfloat16(f[v]);
+      for (int v = 0; v < V; ++v) reinterpret_cast<float*>(&raw)[v] = f[v];
+    } else if constexpr (V == 1) {
+      *reinterpret_cast<bf16*>(&raw) = __float2bfloat16(f[0]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; v += 2) reinterpret_cast<uint32_t*>(&raw)[v / 2] = pack_bf16x2(f[v], f[v + 1]);
     }
   }
 };
@@ -458,321 +471,434 @@ struct Piece {
 template <int V>
 __host__ __device__ constexpr int qk_slots() { return V >= 4 ? 1 : 4 / V; }
 
-// where the pieces of slot sl lie; < 0: behind the head's end
+// where a lane's pieces of a head lie (pa < 0: behind the head's end), and their angles (< 0: not rotated).  Neighbouring lanes'
+// pieces lie next to each other, those of neighbours that rotate too: their pairs lie within a piece.
+struct QkPlace {
+  int pa, pb, angle, angle_b;
+};
 template <int V, bool NEIGH>
-__device__ __forceinline__ void qk_place(const QkArgs& a, int sl, int& pa, int& pb, int& angle) {
+__device__ __forceinline__ QkPlace qk_place(const QkArgs& a, int sl) {
   const int turning = a.rot / (2 * V);
+  QkPlace p;
   if (sl < turning) {
-    pa = NEIGH ? 2 * V * sl : V * sl;
-    pb = NEIGH ? pa + V : pa + a.rot / 2;
-    angle = V * sl;
-  } else {
-    pa = 2 * V * sl;  // = rot + 2 V (sl - turning)
-    pb = pa + V;
-    angle = -1;
-    if (pa >= a.D) pa = -1;
-  }
-}
-
-// the pairs of (x, y) turned by their angles (SIGN -1: back)
-template <int V, bool NEIGH, int SIGN>
-__device__ __forceinline__ void qk_turn(float (&x)[V], float (&y)[V], const float2 (&cs)[V]) {
-  if constexpr (NEIGH && V > 1) {
-#pragma unroll
-    for (int v = 0; v < V; v += 2) {  // the pair of angle v / 2 lies in x, that of angle V / 2 + v / 2 in y
-      const float2 c = cs[v / 2], d = cs[V / 2 + v / 2];
-      const float sx = SIGN * c.y, sy = SIGN * d.y;
-      const float x0 = x[v], x1 = x[v + 1], y0 = y[v], y1 = y[v + 1];
-      x[v] = x0 * c.x - x1 * sx;
-      x[v + 1] = x1 * c.x + x0 * sx;
-      y[v] = y0 * d.x - y1 * sy;
-      y[v + 1] = y1 * d.x + y0 * sy;
+    if (NEIGH && V == 1) {
+      p = {2 * sl, 2 * sl + 1, sl, sl};
+    } else {
+      p.pa = V * sl;
+      p.pb = p.pa + a.rot / 2;
+      p.angle = NEIGH ? p.pa / 2 : p.pa;
+      p.angle_b = NEIGH ? p.pb / 2 : p.pa;
     }
   } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float p = x[v], q = y[v], sn = SIGN * cs[v].y;
-      x[v] = p * cs[v].x - q * sn;
-      y[v] = q * cs[v].x + p * sn;
-    }
+    p.pa = a.rot + V * (sl - turning);
+    p.pb = p.pa + (a.D - a.rot) / 2;
+    p.angle = p.angle_b = -1;
+    if (p.pb >= a.D) p.pa = -1;
   }
+  return p;
 }
 
-// cosines and sines of a token's angles, by a warp, into shared memory, and from there those of the lane's slots
-template <int V, bool NEIGH>
-__device__ __forceinline__ void qk_angles(const QkArgs& a, int b, int t, float2* sm, const int (&angle)[qk_slots<V>()],
-                                          float2 (&cs)[qk_slots<V>()][V]) {
-  const int lane = threadIdx.x & 31;
-  const double p = a.pos ? a.pos[b * a.pos_b + t] : t;
+// An angle's whole turns are of no interest, so turns for each position are kept as a fraction of 64 bits (once for a CTA), and
+// their product with the position as one that wraps around: exact but for the fraction's last bit, times the position.
+__device__ __forceinline__ void qk_turns_of_a_position(const QkArgs& a, unsigned long long* turns) {
+  for (int i = threadIdx.x; i < a.rot / 2; i += blockDim.x) {
+    const double f = a.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
+    turns[i] = (unsigned long long)__double2ll_rn((f - rint(f)) * 18446744073709551616.0);
+  }
+}
+// cosines and sines of a position's angles, by a warp
+__device__ __forceinline__ void qk_angles(const QkArgs& a, const unsigned long long* turns, int pos, float2* sm) {
   __syncwarp();
-  for (int i = lane; i < a.rot / 2; i += 32) {
-    const double turns = p * (a.freqs[i] * 0.15915494309189533577);  // 1 / (2 pi)
+  for (int i = threadIdx.x & 31; i < a.rot / 2; i += 32) {
+    const int part = int((turns[i] * (unsigned long long)(long long)pos) >> 32);  // of 2^32
     float c, s;
-    sincospif(2.f * float(turns - rint(turns)), &s, &c);
+    sincospif(float(part) * 0x1p-31f, &s, &c);
     sm[i] = make_float2(c, s);
   }
   __syncwarp();
-#pragma unroll
-  for (int n = 0; n < qk_slots<V>(); ++n)
-#pragma unroll
-    for (int v = 0; v < V; ++v) cs[n][v] = angle[n] >= 0 ? sm[angle[n] + v] : make_float2(1.f, 0.f);
 }
 
-__device__ __forceinline__ float group_total(float v, int log_g) {
-  for (int o = 1; o < (1 << log_g); o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// The lane's 2 V elements are V pairs of neighbouring registers.  An element's partner is V elements on (halves), or the other
+// of its pair.
+template <int V, bool NEIGH>
+__device__ __forceinline__ float2 qk_partner(const float2 (&z)[V], int j) {
+  if constexpr (NEIGH || V == 1) return make_float2(z[j].y, z[j].x);
+  else return z[(j + V / 2) % V];
+}
+
+// own * A + partner * B: cosines, and sines with the sign of a turn by the angle (SIGN 1) or back (-1), times f
+template <int V, bool NEIGH, int SIGN>
+__device__ __forceinline__ void qk_factors(const float2* sm, const QkPlace& pl, float f, float2 (&A)[V], float2 (&B)[V]) {
+  const float2 none = make_float2(1.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    float2 x, y;  // of elements 2 j and 2 j + 1
+    if constexpr (V == 1) {
+      x = y = pl.angle >= 0 ? sm[pl.angle] : none;
+    } else if constexpr (NEIGH) {
+      x = y = pl.angle >= 0 ? (j < V / 2 ? sm[pl.angle + j] : sm[pl.angle_b + j - V / 2]) : none;
+    } else {
+      x = pl.angle >= 0 ? sm[pl.angle + 2 * j % V] : none;
+      y = pl.angle >= 0 ? sm[pl.angle + (2 * j + 1) % V] : none;
+    }
+    // the first of two partners gets minus the sine in a turn by the angle
+    const float sx = NEIGH || V == 1 || j < V / 2 ? -SIGN : SIGN, sy = NEIGH || V == 1 ? SIGN : j < V / 2 ? -SIGN : SIGN;
+    A[j] = make_float2(x.x * f, y.x * f);
+    B[j] = make_float2(x.y * sx * f, y.y * sy * f);
+  }
+}
+
+// the lane's weights
+template <int V>
+__device__ __forceinline__ void qk_weights(const QkTensor& q, const QkPlace& pl, float2 (&w)[V]) {
+  float* f = reinterpret_cast<float*>(w);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int at = half ? pl.pb : pl.pa;
+    if (!q.w || pl.pa < 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[half * V + v] = 1.f;
+    } else if (V >= 4 && q.wide_w) {
+#pragma unroll
+      for (int v = 0; v + 3 < V; v += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(q.w + at + v);
+        f[half * V + v] = u.x; f[half * V + v + 1] = u.y; f[half * V + v + 2] = u.z; f[half * V + v + 3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[half * V + v] = q.w[at + v];
+    }
+  }
 }
 
 constexpr int QK_WARPS = 4;
 
-template <typename T, int V, bool NEIGH>
-__global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_kernel(const QkArgs a) {
-  constexpr int NS = qk_slots<V>();
-  constexpr int U = NS == 1 ? 4 : 1;  // heads whose loads are on their way together
-  __shared__ float2 sm[QK_WARPS][128];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * QK_WARPS + warp;
-  pdl_wait();
-  pdl_launch();
-  if (item >= (long long)a.B * a.S * a.parts) return;
-  const int part = int(item % a.parts);
-  const long long token = item / a.parts;
-  const int b = int(token / a.S), t = int(token % a.S);
-  int pa[NS], pb[NS], angle[NS];
+// a warp's passes: those of its range, which begins and ends anywhere in a token
+struct QkRange {
+  int p, t, b, left;
+  __device__ __forceinline__ QkRange(const QkArgs& a, const QkTensor& q, int warp) {
+    const int first = warp * q.share + min(warp, q.more), token = first / q.passes;
+    p = first - token * q.passes;
+    b = token / a.S;
+    t = token - b * a.S;
+    left = q.share + (warp < q.more);
+  }
+  // whether the next pass is another token's
+  __device__ __forceinline__ bool next(const QkArgs& a, const QkTensor& q) {
+    --left;
+    if (++p < q.passes) return false;
+    p = 0;
+    if (++t == a.S) {
+      t = 0;
+      ++b;
+    }
+    return true;
+  }
+};
+
+// The passes' pieces on their way through shared memory: a lane copies those that it will use itself, so that nothing but its
+// own copies is waited for.  (In registers a pass or two ahead is all that fits beside the factors; 16 warps of that keep 16 to
+// 32 KB on their way to an SM, and the chain of a pass was exposed.)
+// Pieces of two bytes cannot be copied so and are loaded where they are used.
+template <typename T, int V, bool GRAD>
+struct QkStream {
+  static constexpr int NS = qk_slots<V>(), BYTES = sizeof(T) * V, PIECES = (GRAD ? 4 : 2) * NS;
+  static constexpr bool ASYNC = BYTES >= 4;
+  static constexpr int STAGES = !ASYNC ? 1 : PIECES * BYTES * 32 * 6 <= 8192 ? 6 : 4;
+  static constexpr int SMEM = ASYNC ? STAGES * PIECES * BYTES * 32 : 16;  // of a warp
+  const QkArgs& a;
+  const QkTensor& q;
+  const QkPlace (&at)[NS];
+  uint8_t* ring;
+  QkRange to;
+  int slot = 0, per_pass, sub;
+  const T *src, *grd;
+
+  __device__ __forceinline__ QkStream(const QkArgs& a_, const QkTensor& q_, const QkPlace (&at_)[NS], uint8_t* ring_, const QkRange& range)
+      : a(a_), q(q_), at(at_), ring(ring_ + (threadIdx.x & 31) * BYTES), to(range), per_pass(32 >> a_.log_g), sub((threadIdx.x & 31) >> a_.log_g) {
+    seek();
+#pragma unroll 1
+    for (int s = 0; s < STAGES - 1; ++s) ahead();
+  }
+  __device__ __forceinline__ void seek() {
+    const long long h = to.p * per_pass + sub;
+    src = static_cast<const T*>(q.x) + to.b * q.xb + to.t * q.xt + h * q.xh;
+    if (GRAD) grd = static_cast<const T*>(q.d) + to.b * q.db + to.t * q.dt + h * q.dh;
+  }
+  __device__ __forceinline__ void step() {
+    src += per_pass * q.xh;
+    if (GRAD) grd += per_pass * q.dh;
+    if (to.next(a, q)) seek();
+  }
+  __device__ __forceinline__ void copy(const T* from, int piece) {
+    const uint32_t dst = smem_u32(ring + (slot * PIECES + piece) * BYTES * 32);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+    else if constexpr (ASYNC) asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(BYTES >= 4 ? BYTES : 4) : "memory");
+  }
+  // starts the next pass' copies (an empty group behind the last)
+  __device__ __forceinline__ void ahead() {
+    if constexpr (ASYNC) {
+      if (to.left > 0) {
+        if (to.p * per_pass + sub < q.H) {
 #pragma unroll
-  for (int n = 0; n < NS; ++n) qk_place<V, NEIGH>(a, (lane & ((1 << a.log_g) - 1)) + n * 32, pa[n], pb[n], angle[n]);
-  float2 cs[NS][V];
-  qk_angles<V, NEIGH>(a, b, t, sm[warp], angle, cs);
-  const int per_pass = 32 >> a.log_g, sub = lane >> a.log_g;
-  const float inv_d = 1.f / a.D;
-  int p0 = part * a.per_part, p1 = p0 + a.per_part;
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const QkTensor& q = a.t[which];
-    const int first = max(p0, 0), last = min(p1, q.passes);
-    p0 -= q.passes;
-    p1 -= q.passes;
-    if (first >= last) continue;
-    float wa[NS][V], wb[NS][V];
-#pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        wa[n][v] = (q.w && pa[n] >= 0 ? q.w[pa[n] + v] : 1.f) * q.scale;
-        wb[n][v] = (q.w && pa[n] >= 0 ? q.w[pb[n] + v] : 1.f) * q.scale;
+          for (int n = 0; n < NS; ++n)
+            if (at[n].pa >= 0) {
+              copy(src + at[n].pa, 2 * n);
+              copy(src + at[n].pb, 2 * n + 1);
+              if (GRAD) {
+                copy(grd + at[n].pa, 2 * NS + 2 * n);
+                copy(grd + at[n].pb, 2 * NS + 2 * n + 1);
+              }
+            }
+        }
+        step();
       }
-    const T* src = static_cast<const T*>(q.x) + b * q.xb + t * q.xt;
-    T* dst = static_cast<T*>(q.y) + b * q.yb + t * q.yt;
-    for (int p = first; p < last; p += U) {
-      Piece<T, V> xa[U][NS], xb[U][NS];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = (p + u) * per_pass + sub;
-        const bool in = p + u < last && h < q.H;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          if (in && pa[n] >= 0) {
-            xa[u][n].load(src + h * q.xh + pa[n]);
-            xb[u][n].load(src + h * q.xh + pb[n]);
-          } else {
-            xa[u][n].clear();
-            xb[u][n].clear();
-          }
-        }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+  }
+  // this pass' pieces (`in`: the lane has a head there)
+  __device__ __forceinline__ void take(bool in, float2 (&x)[NS][V], float2 (&g)[NS][V]) {
+    if constexpr (ASYNC) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES >= 2 ? STAGES - 2 : 0) : "memory");
+    const int oldest = slot + 1 >= STAGES ? slot + 1 - STAGES : slot + 1;
+    auto get = [&](int piece, const T* from, bool is, float* f) {
+      Piece<T, V> c;
+      c.clear();
+      if (is) {
+        if constexpr (ASYNC) c.load(reinterpret_cast<const T*>(ring + (oldest * PIECES + piece) * BYTES * 32));
+        else c.load(from);
       }
+      c.get(f);
+    };
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = (p + u) * per_pass + sub;
-        const bool in = p + u < last && h < q.H;
-        float fa[NS][V], fb[NS][V], ss = 0.f;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          xa[u][n].get(fa[n]);
-          xb[u][n].get(fb[n]);
-#pragma unroll
-          for (int v = 0; v < V; ++v) ss += fa[n][v] * fa[n][v] + fb[n][v] * fb[n][v];
-        }
-        const float r = rsqrtf(group_total(ss, a.log_g) * inv_d + a.eps);
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            fa[n][v] = fa[n][v] * r * wa[n][v];
-            fb[n][v] = fb[n][v] * r * wb[n][v];
-          }
-          if (angle[n] >= 0) qk_turn<V, NEIGH, 1>(fa[n], fb[n], cs[n]);
-          if (in && pa[n] >= 0) {
-            xa[u][n].set(fa[n]);
-            xb[u][n].set(fb[n]);
-            xa[u][n].store(dst + h * q.yh + pa[n]);
-            xb[u][n].store(dst + h * q.yh + pb[n]);
-          }
-        }
+    for (int n = 0; n < NS; ++n) {
+      const bool is = in && at[n].pa >= 0;
+      float* f = reinterpret_cast<float*>(x[n]);
+      get(2 * n, src + at[n].pa, is, f);
+      get(2 * n + 1, src + at[n].pb, is, f + V);
+      if (GRAD) {
+        f = reinterpret_cast<float*>(g[n]);
+        get(2 * NS + 2 * n, grd + at[n].pa, is, f);
+        get(2 * NS + 2 * n + 1, grd + at[n].pb, is, f + V);
       }
     }
+    if constexpr (ASYNC) ahead();
+    else step();
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void qk_store(const float2 (&z)[V], const QkPlace& pl, T* dst) {
+  Piece<T, V> a, b;
+  a.set(reinterpret_cast<const float*>(z));
+  b.set(reinterpret_cast<const float*>(z) + V);
+  a.store(dst + pl.pa);
+  b.store(dst + pl.pb);
+}
+
+// position of a token; where there is no such token, that of one that is
+__device__ __forceinline__ int qk_position(const QkArgs& a, int b, int t) {
+  return a.pos ? a.pos[min(b, a.B - 1) * a.pos_b + t] : t;
+}
+
+// The first CTAs take the queries, the others the keys.
+template <typename T, int V, bool NEIGH>
+__global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_kernel(const QkArgs a) {
+  typedef QkStream<T, V, false> Stream;
+  constexpr int NS = qk_slots<V>();
+  __shared__ float2 sm[QK_WARPS][128];
+  __shared__ unsigned long long turns[128];
+  __shared__ __align__(16) uint8_t ring[QK_WARPS][Stream::SMEM];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch();
+  const int which = int(blockIdx.x) >= a.t[0].ctas;
+  const QkTensor& q = a.t[which];
+  QkPlace at[NS];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) at[n] = qk_place<V, NEIGH>(a, (lane & ((1 << a.log_g) - 1)) + n * 32);
+  QkRange now(a, q, (blockIdx.x - (which ? a.t[0].ctas : 0)) * QK_WARPS + warp);
+  int pos = qk_position(a, now.b, now.t);
+  Stream in(a, q, at, ring[warp], now);
+  qk_turns_of_a_position(a, turns);
+  float2 w[NS][V];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) qk_weights<V>(q, at[n], w[n]);
+  __syncthreads();
+  const int per_pass = 32 >> a.log_g, sub = lane >> a.log_g;
+  const float inv_d = 1.f / a.D;
+  while (now.left > 0) {
+    qk_angles(a, turns, pos, sm[warp]);
+    float2 A[NS][V], B[NS][V];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      qk_factors<V, NEIGH, 1>(sm[warp], at[n], q.scale, A[n], B[n]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        A[n][j] = fmul2(A[n][j], w[n][j]);
+        B[n][j] = fmul2(B[n][j], qk_partner<V, NEIGH>(w[n], j));
+      }
+    }
+    T* dst = static_cast<T*>(q.y) + now.b * q.yb + now.t * q.yt + (long long)(now.p * per_pass + sub) * q.yh;
+    pos = now.t + 1 < a.S ? qk_position(a, now.b, now.t + 1) : qk_position(a, now.b + 1, 0);  // the next token's
+    bool over;
+    do {
+      const bool mine = now.p * per_pass + sub < q.H;
+      float2 x[NS][V], ss = make_float2(0.f, 0.f);
+      in.take(mine, x, x);
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int j = 0; j < V; ++j) ss = ffma2(x[n][j], x[n][j], ss);
+      float s = ss.x + ss.y;
+#pragma unroll
+      for (int i = 0; i < 5; ++i)
+        if (i < a.log_g) s += __shfl_xor_sync(0xffffffffu, s, 1 << i);
+      const float r = rsqrtf(s * inv_d + a.eps);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        float2 y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[n][j] = fmul2(x[n][j], make_float2(r, r));  // (first: large elements and weights could overflow)
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = ffma2(qk_partner<V, NEIGH>(x[n], j), B[n][j], fmul2(x[n][j], A[n][j]));
+        if (mine && at[n].pa >= 0) qk_store<T, V>(y, at[n], dst);
+      }
+      dst += per_pass * q.yh;
+      over = now.next(a, q);
+    } while (!over && now.left > 0);
   }
 }
 
 // Backward, with g = the gradient turned back, times the scale, and r = rsqrt(mean(x^2) + eps):
 //   dw_i = sum over tokens and heads of g_i x_i r;  dx = r (g w - x r^2 mean(g w x)).
-// A lane's place in the head is always the same, so the weights' gradients are sums in its registers until the end.
+// A lane's place in the head is always the same: the weights' gradients are sums in its registers until the end.
 template <typename T, int V, bool NEIGH>
 __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_grad_kernel(const QkArgs a) {
+  typedef QkStream<T, V, true> Stream;
   constexpr int NS = qk_slots<V>();
-  constexpr int U = NS == 1 ? 2 : 1;
   __shared__ float2 sm[QK_WARPS][128];
-  __shared__ float red[2][256];
+  __shared__ unsigned long long turns[128];
+  __shared__ float red[256];
+  __shared__ __align__(16) uint8_t ring[QK_WARPS][Stream::SMEM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch();
-  int pa[NS], pb[NS], angle[NS];
+  const int which = int(blockIdx.x) >= a.t[0].ctas;
+  const QkTensor& q = a.t[which];
+  QkPlace at[NS];
 #pragma unroll
-  for (int n = 0; n < NS; ++n) qk_place<V, NEIGH>(a, (lane & ((1 << a.log_g) - 1)) + n * 32, pa[n], pb[n], angle[n]);
+  for (int n = 0; n < NS; ++n) at[n] = qk_place<V, NEIGH>(a, (lane & ((1 << a.log_g) - 1)) + n * 32);
+  QkRange now(a, q, (blockIdx.x - (which ? a.t[0].ctas : 0)) * QK_WARPS + warp);
+  int pos = qk_position(a, now.b, now.t);
+  Stream in(a, q, at, ring[warp], now);
+  qk_turns_of_a_position(a, turns);
+  float2 w[NS][V], dw[NS][V];
+#pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    qk_weights<V>(q, at[n], w[n]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[n][j] = make_float2(0.f, 0.f);
+  }
+  __syncthreads();
   const int per_pass = 32 >> a.log_g, sub = lane >> a.log_g;
   const float inv_d = 1.f / a.D;
-  float da[2][NS][V], db[2][NS][V];
+  while (now.left > 0) {
+    qk_angles(a, turns, pos, sm[warp]);
+    float2 A[NS][V], B[NS][V];
 #pragma unroll
-  for (int w = 0; w < 2; ++w)
+    for (int n = 0; n < NS; ++n) qk_factors<V, NEIGH, -1>(sm[warp], at[n], q.scale, A[n], B[n]);
+    T* dst = static_cast<T*>(q.y) + now.b * q.yb + now.t * q.yt + (long long)(now.p * per_pass + sub) * q.yh;
+    pos = now.t + 1 < a.S ? qk_position(a, now.b, now.t + 1) : qk_position(a, now.b + 1, 0);  // the next token's
+    bool over;
+    do {
+      const bool mine = now.p * per_pass + sub < q.H;
+      float2 x[NS][V], g[NS][V], ss = make_float2(0.f, 0.f), sg = ss;
+      in.take(mine, x, g);
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+      for (int n = 0; n < NS; ++n) {
+        float2 e[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) da[w][n][v] = db[w][n][v] = 0.f;
-  const long long items = (long long)a.B * a.S * a.parts;
-  for (long long item = (long long)blockIdx.x * QK_WARPS + warp; item < items; item += (long long)gridDim.x * QK_WARPS) {
-    const int part = int(item % a.parts);
-    const long long token = item / a.parts;
-    const int b = int(token / a.S), t = int(token % a.S);
-    float2 cs[NS][V];
-    qk_angles<V, NEIGH>(a, b, t, sm[warp], angle, cs);
-    int p0 = part * a.per_part, p1 = p0 + a.per_part;
+        for (int j = 0; j < V; ++j) e[j] = ffma2(qk_partner<V, NEIGH>(g[n], j), B[n][j], fmul2(g[n][j], A[n][j]));
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const QkTensor& q = a.t[which];
-      const int first = max(p0, 0), last = min(p1, q.passes);
-      p0 -= q.passes;
-      p1 -= q.passes;
-      if (first >= last) continue;
-      float wa[NS][V], wb[NS][V];
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          wa[n][v] = q.w && pa[n] >= 0 ? q.w[pa[n] + v] : 1.f;
-          wb[n][v] = q.w && pa[n] >= 0 ? q.w[pb[n] + v] : 1.f;
-        }
-      const T* src = static_cast<const T*>(q.x) + b * q.xb + t * q.xt;
-      const T* grd = static_cast<const T*>(q.d) + b * q.db + t * q.dt;
-      T* dst = static_cast<T*>(q.y) + b * q.yb + t * q.yt;
-      for (int p = first; p < last; p += U) {
-        Piece<T, V> xa[U][NS], xb[U][NS], ga[U][NS], gb[U][NS];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = (p + u) * per_pass + sub;
-          const bool in = p + u < last && h < q.H;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            if (in && pa[n] >= 0) {
-              xa[u][n].load(src + h * q.xh + pa[n]);
-              xb[u][n].load(src + h * q.xh + pb[n]);
-              ga[u][n].load(grd + h * q.dh + pa[n]);
-              gb[u][n].load(grd + h * q.dh + pb[n]);
-            } else {
-              xa[u][n].clear();
-              xb[u][n].clear();
-              ga[u][n].clear();
-              gb[u][n].clear();
-            }
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = (p + u) * per_pass + sub;
-          const bool in = p + u < last && h < q.H;
-          float fa[NS][V], fb[NS][V], ea[NS][V], eb[NS][V], ss = 0.f, sg = 0.f;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            xa[u][n].get(fa[n]);
-            xb[u][n].get(fb[n]);
-            ga[u][n].get(ea[n]);
-            gb[u][n].get(eb[n]);
-            if (angle[n] >= 0) qk_turn<V, NEIGH, -1>(ea[n], eb[n], cs[n]);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              ea[n][v] *= q.scale;
-              eb[n][v] *= q.scale;
-              ss += fa[n][v] * fa[n][v] + fb[n][v] * fb[n][v];
-              sg += fa[n][v] * (ea[n][v] * wa[n][v]) + fb[n][v] * (eb[n][v] * wb[n][v]);
-            }
-          }
-          const float r = rsqrtf(group_total(ss, a.log_g) * inv_d + a.eps);
-          const float m = group_total(sg, a.log_g) * inv_d * r * r;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              da[which][n][v] += ea[n][v] * fa[n][v] * r;
-              db[which][n][v] += eb[n][v] * fb[n][v] * r;
-              fa[n][v] = r * (ea[n][v] * wa[n][v] - fa[n][v] * m);
-              fb[n][v] = r * (eb[n][v] * wb[n][v] - fb[n][v] * m);
-            }
-            if (in && pa[n] >= 0) {
-              xa[u][n].set(fa[n]);
-              xb[u][n].set(fb[n]);
-              xa[u][n].store(dst + h * q.yh + pa[n]);
-              xb[u][n].store(dst + h * q.yh + pb[n]);
-            }
-          }
+        for (int j = 0; j < V; ++j) {
+          g[n][j] = e[j];
+          ss = ffma2(x[n][j], x[n][j], ss);
+          sg = ffma2(fmul2(e[j], w[n][j]), x[n][j], sg);
         }
       }
-    }
+      float s0 = ss.x + ss.y, s1 = sg.x + sg.y;
+#pragma unroll
+      for (int i = 0; i < 5; ++i)
+        if (i < a.log_g) {
+          s0 += __shfl_xor_sync(0xffffffffu, s0, 1 << i);
+          s1 += __shfl_xor_sync(0xffffffffu, s1, 1 << i);
+        }
+      const float r = rsqrtf(s0 * inv_d + a.eps), m = -(s1 * inv_d) * r * r;
+      const float2 r2 = make_float2(r, r), m2 = make_float2(m, m);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        float2 y[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (mine) dw[n][j] = ffma2(g[n][j], fmul2(x[n][j], r2), dw[n][j]);  // (no head: zeros, and with eps = 0 infinitely many of them)
+          y[j] = fmul2(ffma2(x[n][j], m2, fmul2(g[n][j], w[n][j])), r2);
+        }
+        if (mine && at[n].pa >= 0) qk_store<T, V>(y, at[n], dst);
+      }
+      dst += per_pass * q.yh;
+      over = now.next(a, q);
+    } while (!over && now.left > 0);
   }
   // lanes with the same place in other heads, then the warps one after the other
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
+  for (int o = 1 << a.log_g; o < 32; o <<= 1)
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        for (int o = 1 << a.log_g; o < 32; o <<= 1) {
-          da[w][n][v] += __shfl_xor_sync(0xffffffffu, da[w][n][v], o);
-          db[w][n][v] += __shfl_xor_sync(0xffffffffu, db[w][n][v], o);
-        }
-  }
+      for (int j = 0; j < V; ++j) {
+        dw[n][j].x += __shfl_xor_sync(0xffffffffu, dw[n][j].x, o);
+        dw[n][j].y += __shfl_xor_sync(0xffffffffu, dw[n][j].y, o);
+      }
   for (int turn = 0; turn < QK_WARPS; ++turn) {
     if (warp == turn && sub == 0) {
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+      for (int n = 0; n < NS; ++n)
+        if (at[n].pa >= 0) {
+          const float* f = reinterpret_cast<const float*>(dw[n]);
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-          if (pa[n] >= 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              red[w][pa[n] + v] = (turn ? red[w][pa[n] + v] : 0.f) + da[w][n][v];
-              red[w][pb[n] + v] = (turn ? red[w][pb[n] + v] : 0.f) + db[w][n][v];
-            }
+          for (int v = 0; v < V; ++v) {
+            red[at[n].pa + v] = (turn ? red[at[n].pa + v] : 0.f) + f[v];
+            red[at[n].pb + v] = (turn ? red[at[n].pb + v] : 0.f) + f[V + v];
           }
+        }
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 2 * a.D; i += QK_WARPS * 32) a.partial[(long long)blockIdx.x * 2 * a.D + i] = red[i / a.D][i % a.D];
+  for (int i = threadIdx.x; i < a.D; i += QK_WARPS * 32) a.partial[(long long)blockIdx.x * a.D + i] = red[i];
 }
 
-__global__ void __launch_bounds__(256) qk_weight_grad_kernel(const float* partial, float* dqw, float* dkw, int D, int ctas) {
-  const int o = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+// the weights' gradients: the sums of the CTAs' parts, 32 elements of one weight to a CTA, a lane for each
+__global__ void __launch_bounds__(1024) qk_weight_grad_kernel(const float* partial, float* dqw, float* dkw, int D, int q_ctas, int k_ctas) {
+  __shared__ float part[32][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x * 32 + lane, ctas = blockIdx.y ? k_ctas : q_ctas;
+  float* const dst = blockIdx.y ? dkw : dqw;
   pdl_wait();
   pdl_launch();
-  if (o >= 2 * D) return;
-  float* dst = o < D ? dqw : dkw;
   if (!dst) return;
+  const float* src = partial + (blockIdx.y ? (long long)q_ctas * D : 0) + min(i, D - 1);
   float t = 0.f;
-  for (int i = lane; i < ctas; i += 32) t += partial[(long long)i * 2 * D + o];
-  t = warp_total(t);
-  if (lane == 0) dst[o % D] = t;
+#pragma unroll 8
+  for (int c = warp; c < ctas; c += 32) t += src[(long long)c * D];
+  part[warp][lane] = t;
+  __syncthreads();
+  t = warp_total(part[lane][warp]);  // element `warp` of the 32
+  if (lane == 0 && blockIdx.x * 32 + warp < D) dst[blockIdx.x * 32 + warp] = t;
 }
 
-static int qk_ctas(const Ctx* c) { return 4 * c->sm_count; }
+constexpr int QK_MOST = 8;  // CTAs of an SM
+static int qk_ctas(const Ctx* c) { return QK_MOST * c->sm_count; }
 
-// the widest pieces that sizes, strides and addresses allow
+// the widest pieces, up to 16 bytes, that sizes, strides and addresses allow
 static int qk_piece(const QkArgs& a, int elem, bool grad) {
   int V = 16 / elem;
   auto fits = [&](int v) {
@@ -789,29 +915,45 @@ static int qk_piece(const QkArgs& a, int elem, bool grad) {
   return V;
 }
 
-template <typename T, int V, bool GRAD>
-static void launch_qk_one(Ctx* c, QkArgs& a, int neighbours, int grid, cudaStream_t st) {
-  if constexpr (GRAD) {
-    if (neighbours) launch_pdl(qk_norm_rotate_grad_kernel<T, V, true>, dim3(grid), QK_WARPS * 32, 0, st, a);
-    else launch_pdl(qk_norm_rotate_grad_kernel<T, V, false>, dim3(grid), QK_WARPS * 32, 0, st, a);
-  } else {
-    if (neighbours) launch_pdl(qk_norm_rotate_kernel<T, V, true>, dim3(grid), QK_WARPS * 32, 0, st, a);
-    else launch_pdl(qk_norm_rotate_kernel<T, V, false>, dim3(grid), QK_WARPS * 32, 0, st, a);
+// queries and keys get CTAs by their heads and what a token costs besides (about two passes)
+static int qk_divide(Ctx* c, QkArgs& a, int per_sm, int& grid) {
+  const long long tokens = (long long)a.B * a.S;
+  const int all = per_sm * c->sm_count, weigh[2] = {a.t[0].H ? a.t[0].passes + 2 : 0, a.t[1].H ? a.t[1].passes + 2 : 0};
+  grid = 0;
+  for (int i = 0; i < 2; ++i) {
+    QkTensor& q = a.t[i];
+    const int share = q.H ? std::max(1, (int)((long long)(all - 1) * weigh[i] / (weigh[0] + weigh[1]))) : 0;
+    const long long total = tokens * q.passes;
+    if (total > 0x7fffffffll) return fail(c, XFOLD_ERR_ARG, "qk norm: too many tokens");
+    q.ctas = (int)std::min<long long>(share, (total + QK_WARPS - 1) / QK_WARPS);
+    if (q.ctas) {
+      q.share = (int)(total / (q.ctas * QK_WARPS));
+      q.more = (int)(total % (q.ctas * QK_WARPS));
+    }
+    grid += q.ctas;
   }
+  return XFOLD_OK;
 }
 
-template <bool GRAD>
-static void launch_qk_wide(Ctx* c, QkArgs& a, int f32, int V, int neighbours, int grid, cudaStream_t st) {
-  if (f32) {
-    if (V == 4) launch_qk_one<float, 4, GRAD>(c, a, neighbours, grid, st);
-    else if (V == 2) launch_qk_one<float, 2, GRAD>(c, a, neighbours, grid, st);
-    else launch_qk_one<float, 1, GRAD>(c, a, neighbours, grid, st);
-  } else {
-    if (V == 8) launch_qk_one<bf16, 8, GRAD>(c, a, neighbours, grid, st);
-    else if (V == 4) launch_qk_one<bf16, 4, GRAD>(c, a, neighbours, grid, st);
-    else if (V == 2) launch_qk_one<bf16, 2, GRAD>(c, a, neighbours, grid, st);
-    else launch_qk_one<bf16, 1, GRAD>(c, a, neighbours, grid, st);
+template <typename T, int V, bool GRAD>
+static int launch_qk_one(Ctx* c, QkArgs& a, int neighbours, cudaStream_t st) {
+  auto kern = [&] {
+    if constexpr (GRAD) return neighbours ? qk_norm_rotate_grad_kernel<T, V, true> : qk_norm_rotate_grad_kernel<T, V, false>;
+    else return neighbours ? qk_norm_rotate_kernel<T, V, true> : qk_norm_rotate_kernel<T, V, false>;
+  }();
+  static int per_sm[2] = {0, 0};  // resident CTAs
+  int& n = per_sm[neighbours ? 1 : 0];
+  if (!n) {
+    int got = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, QK_WARPS * 32, 0) != cudaSuccess || got < 1)
+      return fail(c, XFOLD_ERR_LAUNCH, "qk norm: occupancy");
+    n = std::min(got, QK_MOST);
   }
+  int grid = 0;
+  if (int rc = qk_divide(c, a, n, grid)) return rc;
+  ProfScope ps(c, XFOLD_K_LAYERNORM, st);
+  launch_pdl(kern, dim3(grid), QK_WARPS * 32, 0, st, a);
+  return check_launch(c, "qk_norm_rotate");
 }
 
 template <bool GRAD>
@@ -819,27 +961,20 @@ static int launch_qk(Ctx* c, QkArgs a, int f32, int neighbours, cudaStream_t st,
   const int V = qk_piece(a, f32 ? 4 : 2, GRAD), slots = (a.D / 2 + V - 1) / V;
   a.log_g = 0;
   while ((1 << a.log_g) < slots && a.log_g < 5) ++a.log_g;
-  int passes = 0;
-  for (QkTensor& q : a.t) {
-    q.passes = (q.H + (32 >> a.log_g) - 1) / (32 >> a.log_g);
-    passes += q.passes;
+  for (QkTensor& q : a.t) q.passes = (q.H + (32 >> a.log_g) - 1) / (32 >> a.log_g);
+  int rc;
+  if (f32) {
+    rc = V == 4 ? launch_qk_one<float, 4, GRAD>(c, a, neighbours, st) : V == 2 ? launch_qk_one<float, 2, GRAD>(c, a, neighbours, st)
+                                                                              : launch_qk_one<float, 1, GRAD>(c, a, neighbours, st);
+  } else {
+    rc = V == 8   ? launch_qk_one<bf16, 8, GRAD>(c, a, neighbours, st)
+         : V == 4 ? launch_qk_one<bf16, 4, GRAD>(c, a, neighbours, st)
+         : V == 2 ? launch_qk_one<bf16, 2, GRAD>(c, a, neighbours, st)
+                  : launch_qk_one<bf16, 1, GRAD>(c, a, neighbours, st);
   }
-  // a warp for each token, or several where that leaves warps without work
-  const long long tokens = (long long)a.B * a.S, want = 16ll * c->sm_count;
-  a.parts = (int)std::max(1ll, std::min<long long>(passes, want / std::max(1ll, tokens)));
-  a.per_part = (passes + a.parts - 1) / a.parts;
-  a.parts = (passes + a.per_part - 1) / a.per_part;
-  const long long ctas = (tokens * a.parts + QK_WARPS - 1) / QK_WARPS;
-  if (ctas > 0x7fffffffll) return fail(c, XFOLD_ERR_ARG, "qk norm: too many tokens");
-  const int grid = GRAD ? (int)std::min<long long>(ctas, qk_ctas(c)) : (int)ctas;
-  {
-    ProfScope ps(c, XFOLD_K_LAYERNORM, st);
-    launch_qk_wide<GRAD>(c, a, f32, V, neighbours, grid, st);
-  }
-  if (int rc = check_launch(c, "qk_norm_rotate")) return rc;
-  if (!dqw && !dkw) return XFOLD_OK;
+  if (rc || (!dqw && !dkw)) return rc;
   ProfScope ps(c, XFOLD_K_LAYERNORM, st);
-  launch_pdl(qk_weight_grad_kernel, dim3((2 * a.D + 7) / 8), 256, 0, st, (const float*)a.partial, dqw, dkw, a.D, grid);
+  launch_pdl(qk_weight_grad_kernel, dim3((a.D + 31) / 32, 2), 1024, 0, st, (const float*)a.partial, dqw, dkw, a.D, a.t[0].ctas, a.t[1].ctas);
   return check_launch(c, "qk_weight_grad_kernel");
 }
 
@@ -861,6 +996,7 @@ static int qk_fill(Ctx* c, const xfold_qk_norm* n, QkArgs& a, bool grad, const c
     t.H = i ? n->Hk : n->Hq;
     t.w = i ? n->k_weight : n->q_weight;
     t.scale = i ? 1.f : n->q_scale;
+    t.wide_w = (uintptr_t)t.w % 16 == 0;
     if (!t.H || !a.B || !a.S) continue;
     if (!x[i]->at || !y[i]->at || (grad && !d[i]->at)) return fail(c, XFOLD_ERR_ARG, "%s: null argument", what);
     t.x = x[i]->at; t.xb = x[i]->batch; t.xt = x[i]->token; t.xh = x[i]->head;
@@ -960,7 +1096,7 @@ int xfold_qk_norm_rotate_fwd(xfold_ctx* cx, const xfold_qk_norm* n, void* stream
 }
 
 size_t xfold_qk_norm_rotate_bwd_workspace_bytes(xfold_ctx* cx, int D) {
-  return cx && D > 0 ? (size_t)qk_ctas(reinterpret_cast<const Ctx*>(cx)) * 2 * D * sizeof(float) : 0;
+  return cx && D > 0 ? (size_t)qk_ctas(reinterpret_cast<const Ctx*>(cx)) * D * sizeof(float) : 0;
 }
 
 int xfold_qk_norm_rotate_bwd(xfold_ctx* cx, const xfold_qk_norm* n, float* dq_weight, float* dk_weight, void* ws, size_t ws_bytes, void* stream) {
