@@ -13,9 +13,10 @@ namespace xf {
 // ---------------------------------------------------------------------------------------------
 // Rows to 8 bits: s = max |x| / 127 (in 32 bits), q = x / s rounded to the nearest whole number, ties to even, exactly.
 //
-// t = x * (1 / s) is within 2e-5 of the quotient.  Where it lies that near to a border between two numbers the residual
-// x - q s decides: it has no more bits than a float32 holds, so the fused multiply-add is exact.
+// One element: t = x * (1 / s) is within 2e-5 of the quotient.  Where it lies that near to a border between two numbers the
+// residual x - q s decides: it has no more bits than a float32 holds, so the fused multiply-add is exact.
 // A row whose scale would be subnormal becomes zeros with scale 0; a row that holds something not finite zeros with scale NaN.
+// Bound by its instructions: nine for an element, and 300 for a warp (8192 x 4096 in 16 bits: 25 us, of which 15 are the bytes').
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ int quantise(float x, float s, float r) {
   const float t = x * r;
@@ -27,44 +28,116 @@ __device__ __forceinline__ int quantise(float x, float s, float r) {
   return int(q);
 }
 
-template <typename T, int V>
-struct RowPiece;  // V elements that are loaded at once
-template <>
-struct RowPiece<bf16, 8> {
-  uint4 u;
-  __device__ __forceinline__ void load(const bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ float at(int i) const {
-    const uint32_t w = i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w;
-    return i & 1 ? bf16_hi(w) : bf16_lo(w);
-  }
-};
-template <>
-struct RowPiece<float, 4> {
-  float4 u;
-  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
-  __device__ __forceinline__ float at(int i) const { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
-};
-template <typename T>
-struct RowPiece<T, 1> {
-  T u;
-  __device__ __forceinline__ void load(const T* p) { u = *p; }
-  __device__ __forceinline__ float at(int) const { return float(u); }
-};
-
 struct QuantArgs {
   const void* x;
   long long ldx, M, ldq;
   int8_t* q;
   float* scale;
   int K, pitch, log_tpr;  // pitch: bytes of a row that are written (zeros from K on); threads for each row
+  int wide_q;             // rows of q start at 8-byte boundaries
 };
 
-constexpr int QUANT_ELEMS = 32;  // of a row, in a thread's registers
+// (a call of its own: rare, and eight times as long as the common way)
+__device__ __noinline__ uint2 quantise_one_by_one(float4 x, float4 y, float s, float r) {
+  const uint32_t lo = __byte_perm(__byte_perm(quantise(x.x, s, r), quantise(x.y, s, r), 0x0040),
+                                  __byte_perm(quantise(x.z, s, r), quantise(x.w, s, r), 0x0040), 0x5410);
+  return make_uint2(lo, __byte_perm(__byte_perm(quantise(y.x, s, r), quantise(y.y, s, r), 0x0040),
+                                    __byte_perm(quantise(y.z, s, r), quantise(y.w, s, r), 0x0040), 0x5410));
+}
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t m;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
+}
+
+// Eight neighbouring elements of a row as they lie in memory.  ALIGNED: rows start at 16-byte boundaries, and K is a multiple of 8.
+template <typename T, bool ALIGNED>
+struct Eight {
+  static constexpr int W = sizeof(T) * 2, PER = 4 / sizeof(T);  // words; elements of a word
+  uint32_t w[W];
+
+  // elements 8 i .. 8 i + 7 of a row; elements from `n` on are zero
+  __device__ __forceinline__ void load(const QuantArgs& a, const T* row, long long i, int n) {
+    const T* at = row + i * 8;
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int g = 0; g < W / 4; ++g) *reinterpret_cast<uint4*>(w + 4 * g) = reinterpret_cast<const uint4*>(at)[g];
+      return;
+    }
+    // the 16-byte pieces around them, and a shift.  Of the first and the last row a piece could reach beyond the array.
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(at), from = addr & ~uintptr_t(15);
+    const uintptr_t first = reinterpret_cast<uintptr_t>(a.x), last = first + ((a.M - 1) * a.ldx + a.K) * sizeof(T);
+    if (from >= first && from + 4 * W + 16 <= last) {
+      uint32_t u[W + 4];
+#pragma unroll
+      for (int g = 0; g < W / 4 + 1; ++g) *reinterpret_cast<uint4*>(u + 4 * g) = reinterpret_cast<const uint4*>(from)[g];
+      const bool two = addr & 8, one = addr & 4;
+#pragma unroll
+      for (int e = 0; e < W + 2; ++e) u[e] = two ? u[e + 2] : u[e];
+#pragma unroll
+      for (int e = 0; e < W + 1; ++e) u[e] = one ? u[e + 1] : u[e];
+#pragma unroll
+      for (int e = 0; e < W; ++e) w[e] = sizeof(T) == 2 ? __funnelshift_r(u[e], u[e + 1], (addr & 2) * 8) : u[e];
+      if (n < 8) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) w[e] = e * PER + PER <= n ? w[e] : e * PER < n ? w[e] & 0xffffu : 0u;
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      w[e] = 0;
+      if constexpr (sizeof(T) == 2) {
+        if (2 * e < n) w[e] = reinterpret_cast<const uint16_t*>(at)[2 * e];
+        if (2 * e + 1 < n) w[e] |= uint32_t(reinterpret_cast<const uint16_t*>(at)[2 * e + 1]) << 16;
+      } else if (e < n) {
+        w[e] = reinterpret_cast<const uint32_t*>(at)[e];
+      }
+    }
+  }
+  // the largest magnitude's bits so far (in 16 bits: of the elements at even and odd places)
+  __device__ __forceinline__ void most(uint32_t& m) const {
+#pragma unroll
+    for (int e = 0; e < W; ++e) m = sizeof(T) == 2 ? max_u16x2(m, w[e] & 0x7fff7fffu) : max(m, w[e] & 0x7fffffffu);
+  }
+  __device__ __forceinline__ float2 pair(int j) const {
+    if constexpr (sizeof(T) == 2) return make_float2(bf16_lo(w[j]), bf16_hi(w[j]));
+    else return make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+  }
+  // All eight quantised.  Added to 1.5 * 2^23 a product is rounded to a whole number, whose low bits are the sum's: t from x r,
+  // corrected by what the quotient differs from it, d = x (r + r_low) - t, which rounds two times at 2^-25.  Where d is that near
+  // to a half the eight are taken one by one.  (Without r_low, within 1e-4 of a half, half the warps with 16-bit numbers would:
+  // their quotients by the largest of them are near to halves often.)
+  __device__ __forceinline__ uint2 quantised(float s, float r, float r_low, float near) const {
+    constexpr float BIG = 12582912.f;
+    const float2 big = make_float2(BIG, BIG), minus = make_float2(-1.f, -1.f), r2 = make_float2(r, r), l2 = make_float2(r_low, r_low),
+                 quarter = make_float2(-0.25f, -0.25f);
+    uint32_t q[8];
+    float least = 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 x = pair(j), t = ffma2(x, r2, big), d = ffma2(x, l2, ffma2(x, r2, ffma2(t, minus, big))), y = fadd2(t, d);
+      const float2 e = ffma2(d, d, quarter);  // near to a half: d's distance to it
+      least = fminf(least, fminf(fabsf(e.x), fabsf(e.y)));
+      q[2 * j] = __float_as_uint(y.x);
+      q[2 * j + 1] = __float_as_uint(y.y);
+    }
+    if (least < near) {
+      const float2 u = pair(0), v = pair(1), x = pair(2), y = pair(3);
+      return quantise_one_by_one(make_float4(u.x, u.y, v.x, v.y), make_float4(x.x, x.y, y.x, y.y), s, r);
+    }
+    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
+  }
+};
+
+template <typename T>
+constexpr int QUANT_PIECES = 8 / sizeof(T);  // of eight elements of a row, in 16 of a thread's registers (32: long batches a tenth faster, others slower)
 
 // `HELD`: the row stays in registers between the two passes over it
-template <typename T, int V, bool HELD>
+template <typename T, bool ALIGNED, bool HELD>
 __global__ void __launch_bounds__(1024) quantise_rows_kernel(const QuantArgs a) {
-  constexpr int NV = QUANT_ELEMS / V;
   __shared__ uint32_t part[32];
   const int tpr = 1 << a.log_tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x >> a.log_tpr;
   const long long m = (long long)blockIdx.x * rows + (threadIdx.x >> a.log_tpr);
@@ -72,32 +145,30 @@ __global__ void __launch_bounds__(1024) quantise_rows_kernel(const QuantArgs a) 
   pdl_launch();
   const bool in = m < a.M;
   const T* x = static_cast<const T*>(a.x) + (in ? m : 0) * a.ldx;
-  const int nv = in ? a.K / V : 0;  // (V > 1: K is a multiple of V)
-  RowPiece<T, V> p[NV];
+  const int pieces = in ? (a.K + 7) / 8 : 0;
+  Eight<T, ALIGNED> p[HELD ? QUANT_PIECES<T> : 1];
   uint32_t most = 0;  // of the magnitudes' bits: orders floats, with what is not finite on top
   if constexpr (HELD) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (t + i * tpr < nv) p[i].load(x + (long long)(t + i * tpr) * V);
+    for (int i = 0; i < QUANT_PIECES<T>; ++i)
+      if (t + i * tpr < pieces) p[i].load(a, x, t + i * tpr, a.K - (t + i * tpr) * 8);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (t + i * tpr < nv) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) most = max(most, __float_as_uint(p[i].at(v)) & 0x7fffffffu);
-      }
+    for (int i = 0; i < QUANT_PIECES<T>; ++i)
+      if (t + i * tpr < pieces) p[i].most(most);
   } else {
-    for (int i = t; i < nv; i += tpr) {
-      p[0].load(x + (long long)i * V);
-#pragma unroll
-      for (int v = 0; v < V; ++v) most = max(most, __float_as_uint(p[0].at(v)) & 0x7fffffffu);
+    for (int i = t; i < pieces; i += tpr) {
+      p[0].load(a, x, i, a.K - i * 8);
+      p[0].most(most);
     }
   }
+  if (sizeof(T) == 2) most = max(most & 0xffffu, most >> 16) << 16;
   most = __reduce_max_sync(0xffffffffu, most);
   if (tpr > 32) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
     __syncthreads();
     const int w0 = (threadIdx.x >> a.log_tpr) << (a.log_tpr - 5);
     most = 0;
+#pragma unroll 4
     for (int w = 0; w < tpr / 32; ++w) most = max(most, part[w0 + w]);
   }
   if (!in) return;
@@ -105,55 +176,51 @@ __global__ void __launch_bounds__(1024) quantise_rows_kernel(const QuantArgs a) 
   const bool fine = most < 0x7f800000u, some = fine && s >= FLT_MIN;
   if (!some) s = fine ? 0.f : __uint_as_float(0x7fffffffu);
   r = some ? 1.f / s : 0.f;
+  const bool low = some && s < 1e20f;  // (r_low of larger scales would be subnormal)
+  const float r_low = low ? fmaf(-r, s, 1.f) * r : 0.f, near = low ? 1.2e-7f : 1e-4f;
   if (t == 0) a.scale[m] = s;
   int8_t* q = a.q + m * a.ldq;
-  auto put = [&](const RowPiece<T, V>& pc, int i) {
-    if constexpr (V == 1) {
-      q[i] = int8_t(some ? quantise(pc.at(0), s, r) : 0);
+  auto put = [&](uint2 w, int i) {
+    if (a.wide_q) {
+      *reinterpret_cast<uint2*>(q + (long long)i * 8) = w;
     } else {
-      uint32_t w[V / 4];
-#pragma unroll
-      for (int g = 0; g < V / 4; ++g) {
-        w[g] = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[g] |= uint32_t((some ? quantise(pc.at(4 * g + e), s, r) : 0) & 255) << (8 * e);
-      }
-      if constexpr (V == 8) *reinterpret_cast<uint2*>(q + (long long)i * 8) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(q + (long long)i * 4) = w[0];
+      for (int e = 0; e < 8 && i * 8 + e < a.pitch; ++e) q[i * 8 + e] = int8_t((e < 4 ? w.x : w.y) >> (e & 3) * 8);
     }
   };
   if constexpr (HELD) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (t + i * tpr < nv) put(p[i], t + i * tpr);
+    for (int i = 0; i < QUANT_PIECES<T>; ++i)
+      if (t + i * tpr < pieces) put(some ? p[i].quantised(s, r, r_low, near) : make_uint2(0, 0), t + i * tpr);
   } else {
-    for (int i = t; i < nv; i += tpr) {
-      p[0].load(x + (long long)i * V);
-      put(p[0], i);
+    for (int i = t; i < pieces; i += tpr) {
+      p[0].load(a, x, i, a.K - i * 8);
+      put(some ? p[0].quantised(s, r, r_low, near) : make_uint2(0, 0), i);
     }
   }
-  for (int i = a.K + t; i < a.pitch; i += tpr) q[i] = 0;
+  for (int i = pieces + t; i * 8 < a.pitch; i += tpr) put(make_uint2(0, 0), i);
 }
 
-template <typename T, int V>
-static void launch_quantise_wide(QuantArgs a, cudaStream_t st) {
+template <typename T>
+static void launch_quantise_of(QuantArgs a, bool aligned, cudaStream_t st) {
   a.log_tpr = 5;
-  while ((1 << a.log_tpr) * QUANT_ELEMS < a.K && a.log_tpr < 10) ++a.log_tpr;
-  const bool held = (1 << a.log_tpr) * QUANT_ELEMS >= a.K;
+  while ((1 << a.log_tpr) * QUANT_PIECES<T> * 8 < a.K && a.log_tpr < 10) ++a.log_tpr;
+  const bool held = (1 << a.log_tpr) * QUANT_PIECES<T> * 8 >= a.K;
   const int threads = std::max(128, 1 << a.log_tpr), rows = threads >> a.log_tpr;
   const unsigned grid = (unsigned)((a.M + rows - 1) / rows);
-  if (held) launch_pdl(quantise_rows_kernel<T, V, true>, dim3(grid), threads, 0, st, a);
-  else launch_pdl(quantise_rows_kernel<T, V, false>, dim3(grid), threads, 0, st, a);
+  auto kern = aligned ? (held ? quantise_rows_kernel<T, true, true> : quantise_rows_kernel<T, true, false>)
+                      : (held ? quantise_rows_kernel<T, false, true> : quantise_rows_kernel<T, false, false>);
+  launch_pdl(kern, dim3(grid), threads, 0, st, a);
 }
 
+// pitch: a multiple of 8 where rows of q start at 8-byte boundaries
 static int launch_quantise(Ctx* c, const void* x, int f32, long long ldx, long long M, int K, int8_t* q, long long ldq, int pitch, float* scale,
                            cudaStream_t st) {
-  QuantArgs a{x, ldx, M, ldq, q, scale, K, pitch, 0};
-  const int wide = f32 ? 4 : 8;
-  const bool vec = K % wide == 0 && ldx % wide == 0 && (uintptr_t)x % 16 == 0 && ldq % wide == 0 && (uintptr_t)q % wide == 0;
+  QuantArgs a{x, ldx, M, ldq, q, scale, K, pitch, 0, 0};
+  const bool aligned = K % 8 == 0 && (uintptr_t)x % 16 == 0 && (M == 1 || ldx * (f32 ? 4 : 2) % 16 == 0);
+  a.wide_q = (uintptr_t)q % 8 == 0 && (M == 1 || ldq % 8 == 0) && pitch % 8 == 0;
   ProfScope ps(c, XFOLD_K_LAYERNORM, st);
-  if (f32) vec ? launch_quantise_wide<float, 4>(a, st) : launch_quantise_wide<float, 1>(a, st);
-  else vec ? launch_quantise_wide<bf16, 8>(a, st) : launch_quantise_wide<bf16, 1>(a, st);
+  if (f32) launch_quantise_of<float>(a, aligned, st);
+  else launch_quantise_of<bf16>(a, aligned, st);
   return check_launch(c, "quantise_rows_kernel");
 }
 
@@ -468,6 +535,8 @@ static int i8_product(Ctx* c, const int8_t* x, long long ldx, const float* x_sca
 }
 
 static long long pad16(long long k) { return (k + 15) & ~15ll; }
+// distance of quantised rows: whole sectors of the L2 (5000^3: 142 us at rows 5008 bytes apart, 127 at 5056)
+static long long pad64(long long k) { return (k + 63) & ~63ll; }
 
 }  // namespace xf
 
@@ -486,7 +555,7 @@ int xfold_quantize_rows_fwd(xfold_ctx* cx, const void* x, int is_f32, long long 
   if (!x || !q || !scale || ldx < K || (uintptr_t)x % (is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "quantise rows: null or misaligned argument");
   if (ldq < K) return fail(c, XFOLD_ERR_ARG, "quantise rows: rows of the result are too near to each other");
   DeviceGuard dev(c);
-  return launch_quantise(c, x, is_f32, ldx, M, K, (int8_t*)q, ldq, (int)std::min(ldq, pad16(K)), scale, (cudaStream_t)stream);
+  return launch_quantise(c, x, is_f32, ldx, M, K, (int8_t*)q, ldq, (int)std::min(ldq, pad64(K)), scale, (cudaStream_t)stream);
 }
 
 int xfold_linear_int8_quantized_fwd(xfold_ctx* cx, const void* x, long long ldx, const float* x_scale, long long M, int K, const void* w,
@@ -503,7 +572,7 @@ int xfold_linear_int8_quantized_fwd(xfold_ctx* cx, const void* x, long long ldx,
 }
 
 size_t xfold_linear_int8_workspace_bytes(long long M, int K) {
-  return M > 0 && K > 0 ? align_up((size_t)M * pad16(K), 1024) + align_up((size_t)M * 4, 1024) + 1024 : 0;
+  return M > 0 && K > 0 ? align_up((size_t)M * pad64(K), 1024) + align_up((size_t)M * 4, 1024) + 1024 : 0;
 }
 
 int xfold_linear_int8_fwd(xfold_ctx* cx, const void* x, int is_f32, long long ldx, long long M, int K, const void* w, long long ldw, int N,
@@ -517,7 +586,7 @@ int xfold_linear_int8_fwd(xfold_ctx* cx, const void* x, int is_f32, long long ld
   if (is_f32 != 0 && is_f32 != 1) return fail(c, XFOLD_ERR_ARG, "int8 linear: type");
   if (!x || ldx < K || (uintptr_t)x % (is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "int8 linear: null or misaligned activations");
   Carver cv(ws, ws_bytes);
-  int8_t* q = (int8_t*)cv.take((size_t)M * pad16(K));
+  int8_t* q = (int8_t*)cv.take((size_t)M * pad64(K));
   float* scale = (float*)cv.take((size_t)M * 4);
   if (!ws || (uintptr_t)ws % 16 || !cv.ok()) return fail(c, XFOLD_ERR_ARG, "int8 linear: workspace too small (%zu < %zu) or misaligned", ws_bytes, cv.off);
   // what the product would refuse is refused before the first launch
@@ -525,9 +594,9 @@ int xfold_linear_int8_fwd(xfold_ctx* cx, const void* x, int is_f32, long long ld
   if (!w_scale || !out || ldo < N || (uintptr_t)out % (out_is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "int8 linear: scales and result");
   DeviceGuard dev(c);
   cudaStream_t st = (cudaStream_t)stream;
-  if (int rc = launch_quantise(c, x, is_f32, ldx, M, K, q, pad16(K), (int)pad16(K), scale, st)) return rc;
+  if (int rc = launch_quantise(c, x, is_f32, ldx, M, K, q, pad64(K), (int)pad16(K), scale, st)) return rc;
   // the quantisation starts behind what wrote the weights, and the product is launched behind its start
-  return i8_product(c, q, pad16(K), scale, M, K, (const int8_t*)w, ldw, N, w_scale, bias, out, out_is_f32, ldo, 1, st);
+  return i8_product(c, q, pad64(K), scale, M, K, (const int8_t*)w, ldw, N, w_scale, bias, out, out_is_f32, ldo, 1, st);
 }
 
 }  // extern "C"

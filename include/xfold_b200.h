@@ -298,7 +298,7 @@ int xfold_qk_norm_rotate_bwd(xfold_ctx* ctx, const xfold_qk_norm* n, float* dq_w
 
 /* ---- linear layers in 8-bit integers (no counterpart in the reference) --------------------------------
  * Rows to 8 bits: scale[m] = max_k |x[m][k]| / 127 in float32, q[m][k] = x[m][k] / scale[m] rounded to the nearest whole
- * number (ties to even; exact).  x bf16 or float32; q int8, rows ldq apart, zeros from K to the next multiple of 16 (as far as
+ * number (ties to even; exact).  x bf16 or float32; q int8, rows ldq apart, zeros from K to the next multiple of 64 (as far as
  * ldq leaves room).  Rows whose scale would be subnormal: zeros, scale 0; rows that hold something not finite: scale NaN. */
 int xfold_quantize_rows_fwd(xfold_ctx* ctx, const void* x, int is_f32, long long ldx, long long M, int K, void* q, long long ldq,
                             float* scale, void* stream);
