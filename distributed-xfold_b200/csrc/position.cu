@@ -146,29 +146,29 @@ static void launch_rel_fwd(Ctx* c, RelFwdArgs a, cudaStream_t st) {
 // ---------------------------------------------------------------------------------------------
 // Gradient of the table: dtable[b][h] = sum over (i, j) with b(i, j) = b of grad[h][i][j].
 //
-// A warp keeps 32 V columns of one head, V neighbours to a lane, and goes down its rows.  Of each 32 columns (a group of
-// lanes) a row's entries lie before the reach, behind it or in another group of tokens, all of them: then a lane adds its V to
-// one of three sums in registers, at two dozen instructions for 512 bytes.  Or they do not: a band along the diagonal.  Its
-// rows are put into shared memory and taken a column to a lane, into sums [nb + 2][32 lanes] of the warp's (a lane's bank is its
-// own: no conflicts, no atomics, and the order of the sum is always the same).
-// The rows of a CTA lie `slices` apart, so that every warp has its share of the band.  CTAs leave their sums in the workspace; a
-// second kernel adds them.
+// A warp keeps 32 V columns of one head, V neighbours to a lane, and goes down its rows, eight at a time.  Of each 32 columns (a
+// group of lanes) the eight rows' entries lie before the reach, behind it or in another group of tokens, all of them: then a
+// lane adds its V to one of three sums in registers.  Or they do not: a band along the diagonal.  Its rows are put into shared
+// memory and taken a column to a lane, into sums [nb + 2][32 lanes] of the warp's (a lane's bank is its own: no conflicts, no
+// atomics, and the order of the sum is always the same).
+// The eights of a CTA lie `slices` apart, so that every warp has its share of the band.  CTAs leave their sums in the workspace;
+// a second kernel adds them.
 // ---------------------------------------------------------------------------------------------
 struct RelBwdArgs {
   RelShared s;
   const void* grad;
   long long sh, sq;       // strides of heads and queries, in elements
   float* partial;         // [H][slices][nb]
-  int slices;             // CTAs for each head: rows slice, slice + slices, ...
-  int cblocks, row_sets;  // blocks of 32 V columns; sets of rows that warps take such a block in
+  int slices;             // CTAs for each head: eights of rows slice, slice + slices, ...
+  int cblocks, row_sets;  // blocks of 32 V columns; sets of eights that warps take such a block in
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
 
-constexpr int REL_ROWS = 8, REL_HALF = 4;  // rows of a warp that are on their way together; that lie in shared memory
+constexpr int REL_ROWS = 8, REL_HALF = 4;  // rows that are on their way together; that lie in shared memory
 template <int V>
-__host__ __device__ constexpr size_t rel_bwd_warp_bytes() { return REL_HALF * 512 + 32 * V * 8; }  // rows; columns' positions, groups
+__host__ __device__ constexpr size_t rel_bwd_warp_bytes() { return REL_HALF * 512 + REL_ROWS * 16 + 32 * V * 8; }  // rows; what is known of them; columns' positions, groups
 
 // sum of a piece
 __device__ __forceinline__ float piece_sum(const RelPiece<float, 4>& p) { return (p.e[0] + p.e[1]) + (p.e[2] + p.e[3]); }
@@ -189,8 +189,9 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) rel_bias_grad_kernel(const R
   const RelShared& s = a.s;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hrows = s.nb + 2;
   uint8_t* own = smem_raw + warp * rel_bwd_warp_bytes<V>();
-  E* srow = reinterpret_cast<E*>(own);  // [REL_HALF][W]
-  int* skp = reinterpret_cast<int*>(own + REL_HALF * 512);
+  E* srow = reinterpret_cast<E*>(own);                        // [REL_HALF][W]
+  int4* sinfo = reinterpret_cast<int4*>(own + REL_HALF * 512);  // of a row: where its buckets end, what makes a place in the lut, group
+  int* skp = reinterpret_cast<int*>(sinfo + REL_ROWS);
   int* skg = skp + W;
   float* sums = reinterpret_cast<float*>(smem_raw + warps * rel_bwd_warp_bytes<V>());
   uint16_t* lut = reinterpret_cast<uint16_t*>(sums + (size_t)warps * hrows * 32);
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) rel_bias_grad_kernel(const R
   pdl_wait();
   pdl_launch();
   const int h = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-  const int rows = (s.Sq - slice + a.slices - 1) / a.slices;  // of this CTA
+  const int eights = ((s.Sq + REL_ROWS - 1) / REL_ROWS - slice + a.slices - 1) / a.slices;  // of this CTA
   const E* g0 = static_cast<const E*>(a.grad) + (long long)h * a.sh;
   float before = 0.f, behind = 0.f, others = 0.f;
   bool staged = false;  // (the table of buckets and the sums are made while the first unit's rows are on their way)
@@ -210,28 +211,34 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) rel_bias_grad_kernel(const R
   };
   for (int unit = warp; unit < a.cblocks * a.row_sets; unit += warps) {
     const int c0 = unit % a.cblocks * W, set = unit / a.cblocks, c1 = c0 + lane * V;
+    const bool mine = c1 < s.Sk;
     RelPiece<E, V> x[REL_ROWS];
-    int qp = 0, qg = 0;  // lane u: of row u of the batch
-    const E* next = g0 + ((long long)set * a.slices + slice) * a.sq + (VEC && c1 < s.Sk ? c1 : 0);
-    const long long step = (long long)a.row_sets * a.slices * a.sq;
-    auto load = [&](int n0) {  // rows n0, n0 + row_sets, ..; rows and columns beyond the last are read as the last, and not added
-      const int last = (rows - 1 - n0) / a.row_sets;
+    int qp = 0, qg = 0;  // lane u: of row u of the eight
+    auto first = [&](int n) { return (n * a.slices + slice) * REL_ROWS; };
+    auto load_row = [&](int u, int i) {  // row i; zeros where there is none
+      const E* row = g0 + (long long)i * a.sq;
+      if constexpr (VEC) {
+        x[u] = RelPiece<E, V>{};
+        if (i < s.Sq && mine) x[u] = *reinterpret_cast<const RelPiece<E, V>*>(row + c1);
+      } else {
 #pragma unroll
-      for (int u = 0; u < REL_ROWS; ++u) {
-        const E* row = next + min(u, last) * step;
-        if constexpr (VEC) {
-          x[u] = *reinterpret_cast<const RelPiece<E, V>*>(row);
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) x[u].e[v] = row[min(c0 + v * 32 + lane, s.Sk - 1)];
+        for (int v = 0; v < V; ++v) {
+          const int j = c0 + v * 32 + lane;
+          x[u].e[v] = E(0.f);
+          if (i < s.Sq && j < s.Sk) x[u].e[v] = row[j];
         }
       }
-      next += REL_ROWS * step;
-      const int i = min(n0 + (lane & (REL_ROWS - 1)) * a.row_sets, rows - 1) * a.slices + slice;
+    };
+    auto load_positions = [&](int i0) {  // (behind the last row: the last one's)
+      const int i = min(i0 + (lane & (REL_ROWS - 1)), s.Sq - 1);
       qp = s.q_pos[i];
       if (GROUPS) qg = s.q_grp[i];
     };
-    if (set < rows) load(set);
+    if (set < eights) {
+#pragma unroll
+      for (int u = 0; u < REL_ROWS; ++u) load_row(u, first(set) + u);
+      load_positions(first(set));
+    }
     __syncwarp();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -255,58 +262,61 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) rel_bias_grad_kernel(const R
     }
     const bool fits = hi <= 0x7fffffff - s.reach && lo >= s.reach - 0x7fffffff;  // (else as a band)
     const int after = fits ? hi + s.reach : 0, until = fits ? lo - s.reach : 0;
-    const bool mine = c1 < s.Sk, same = grp == gmax && fits;
-    for (int n0 = set; n0 < rows; n0 += REL_ROWS * a.row_sets) {
-      const int bp = qp, bg = qg;
+    const bool same = grp == gmax && fits;
+    for (int n = set; n < eights; n += a.row_sets) {
+      const int pmin = __reduce_min_sync(0xffffffffu, qp), pmax = __reduce_max_sync(0xffffffffu, qp);
+      // (all lanes take part in these: none of them behind a condition)
+      const int g = GROUPS ? __reduce_min_sync(0xffffffffu, qg) : 0, g_most = GROUPS ? __reduce_max_sync(0xffffffffu, qg) : 0;
+      const bool one = same && g == g_most, other = GROUPS && one && grp != g;
+      const bool beh = one && !other && until >= pmax, bef = one && !other && !beh && after <= pmin;
+      uint32_t band = __ballot_sync(0xffffffffu, mine && !other && !beh && !bef);
+      if (band) {
+        if (lane < REL_ROWS) sinfo[lane] = make_int4(low_end(qp, s.reach), high_end(qp, s.reach), int(unsigned(s.reach) - unsigned(qp)), qg);
+      }
+      const int i0 = n + a.row_sets < eights ? first(n + a.row_sets) : s.Sq;  // the next rows
+      load_positions(i0);
+      float t = 0.f;
 #pragma unroll
       for (int half = 0; half < REL_ROWS; half += REL_HALF) {
-        uint32_t band = 0;  // lane u: the lanes of row u whose columns lie in the band
 #pragma unroll
         for (int u = half; u < half + REL_HALF; ++u) {
-          if (n0 + u * a.row_sets < rows) {
-            const int p = __shfl_sync(0xffffffffu, bp, u), g = GROUPS ? __shfl_sync(0xffffffffu, bg, u) : 0;
-            const bool other = GROUPS && same && grp != g, in = same && (!GROUPS || grp == g), bef = in && after <= p, beh = in && until >= p;
-            const bool out = other || bef || beh;
-            const uint32_t b = __ballot_sync(0xffffffffu, mine && !out);
-            E* row = srow + (u - half) * W;
-            if constexpr (!VEC) {  // a lane's columns lie apart: everything passes through shared memory
+          E* row = srow + (u - half) * W;
+          if constexpr (!VEC) {  // a lane's columns lie apart: everything passes through shared memory
 #pragma unroll
-              for (int v = 0; v < V; ++v) row[v * 32 + lane] = x[u].e[v];
-              __syncwarp();
-              x[u] = *reinterpret_cast<const RelPiece<E, V>*>(row + lane * V);
-#pragma unroll
-              for (int v = 0; v < V; ++v)
-                if (c1 + v >= s.Sk) x[u].e[v] = E(0.f);
-            } else if (b) {
-              *reinterpret_cast<RelPiece<E, V>*>(row + lane * V) = x[u];
-            }
-            const float t = mine ? piece_sum(x[u]) : 0.f;
-            if (beh) behind += t;  // (with a reach of nothing a key at the query's own position is on both sides)
-            else if (bef) before += t;
-            if (GROUPS && other) others += t;
-            if (lane == u) band = b;
+            for (int v = 0; v < V; ++v) row[v * 32 + lane] = x[u].e[v];
+            __syncwarp();
+            t += piece_sum(*reinterpret_cast<const RelPiece<E, V>*>(row + lane * V));
+          } else {
+            if (band) *reinterpret_cast<RelPiece<E, V>*>(row + lane * V) = x[u];
+            t += piece_sum(x[u]);
           }
+          load_row(u, i0 + u);
         }
-        __syncwarp();
-        if (half + REL_HALF == REL_ROWS && n0 + REL_ROWS * a.row_sets < rows) load(n0 + REL_ROWS * a.row_sets);
-        uint32_t todo = __ballot_sync(0xffffffffu, band != 0);
-        while (todo) {
-          const int u = __ffs(todo) - 1;
-          todo &= todo - 1;
-          const int p = __shfl_sync(0xffffffffu, bp, u), g = GROUPS ? __shfl_sync(0xffffffffu, bg, u) : 0;
-          const int low = low_end(p, s.reach), high = high_end(p, s.reach);
-          const E* row = srow + (u - half) * W + lane;
-          uint32_t b = __shfl_sync(0xffffffffu, band, u);
+        if (band) {
+          __syncwarp();
+          uint32_t left = band;
           do {
-            const int at = (__ffs(b) - 1) / SHARE * 32;  // the first 32 columns left
-            b &= ~(((1u << SHARE) - 1) << (at / 32 * SHARE));
-            int k = lut[min(max(skp[at + lane], low), high) - p + s.reach];
-            if (GROUPS && skg[at + lane] != g) k = (s.nb - 1) * 32;
-            if (c0 + at + lane < s.Sk) acc[k] += to_float(row[at]);
-          } while (b);
+            const int at = (__ffs(left) - 1) / SHARE * 32 + lane;  // this lane's of the first 32 columns left
+            left &= ~(((1u << SHARE) - 1) << (at / 32 * SHARE));
+            const int kp = skp[at], kg = GROUPS ? skg[at] : 0;
+            int k[REL_HALF];
+            float v[REL_HALF];
+#pragma unroll
+            for (int u = 0; u < REL_HALF; ++u) {
+              const int4 r = sinfo[half + u];
+              k[u] = lut[unsigned(min(max(kp, r.x), r.y)) + unsigned(r.z)];
+              if (GROUPS && kg != r.w) k[u] = (s.nb - 1) * 32;
+              v[u] = to_float(srow[u * W + at]);
+            }
+#pragma unroll
+            for (int u = 0; u < REL_HALF; ++u) acc[k[u]] += v[u];
+          } while (left);
         }
         __syncwarp();
       }
+      before += bef ? t : 0.f;
+      behind += beh ? t : 0.f;
+      if (GROUPS) others += other ? t : 0.f;
     }
   }
   if (!staged) stage();
@@ -348,7 +358,7 @@ struct RelBwdPlan {
 // CTAs for each head: three or two to an SM, by their registers and their sums' room
 static int rel_bwd_slices(int nb, int H, int Sq, bool vec, int sms) {
   const int per_sm = vec && (size_t)(nb + 2) * 128 * 8 <= 36 * 1024 ? 3 : 2;
-  return std::max(1, std::min(per_sm * sms / H, (Sq + 7) / 8));
+  return std::max(1, std::min(per_sm * sms / H, (Sq + REL_ROWS - 1) / REL_ROWS));
 }
 static RelBwdPlan rel_bwd_plan(int nb, int H, int Sq, int Sk, int reach, int V, bool vec, int sms) {
   RelBwdPlan p;
@@ -358,11 +368,11 @@ static RelBwdPlan rel_bwd_plan(int nb, int H, int Sq, int Sk, int reach, int V, 
   p.smem = p.warps * per_warp + rest;
   p.slices = rel_bwd_slices(nb, H, Sq, vec, sms);
   p.cblocks = (Sk + 32 * V - 1) / (32 * V);
-  // sets of rows: the warps' rounds over the units are to come out even, but a unit costs about as much as four rows to begin
-  const int rows = (Sq + p.slices - 1) / p.slices;
+  // sets of rows: the warps' rounds over the units are to come out even, but a unit costs about as much as half an eight to begin
+  const int eights = ((Sq + REL_ROWS - 1) / REL_ROWS + p.slices - 1) / p.slices;
   double best = 1e30;
   for (int n = 1; n <= 8; n *= 2) {
-    const double cost = double((p.cblocks * n + p.warps - 1) / p.warps) * ((rows + n - 1) / n + 4);
+    const double cost = double((p.cblocks * n + p.warps - 1) / p.warps) * ((eights + n - 1) / n + 0.5);
     if (cost < best) {
       best = cost;
       p.row_sets = n;
