@@ -203,6 +203,10 @@ def _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale):
     return dev, (b, s, hq, hk, d, rot, bool(inter), dt is F32, qw, kw, freqs, pos, pos_b, eps, q_scale, *at_q, *at_k)
 
 
+def _new(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)   # (half the host time of new_empty)
+
+
 def _weight(w: torch.Tensor, d: int) -> int:
     if w.dtype is not F32 or w.shape != (d,) or (w.stride(0) != 1 and d > 1):
         _refuse("norm weights: float32 [width]")
@@ -218,7 +222,7 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, which may be the inputs."""
     dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
     if out is None:
-        qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+        qo, ko = _new(q), _new(k)
     else:
         qo, ko = out
         for o, x in ((qo, q), (ko, k)):
@@ -248,8 +252,9 @@ def norm_rotate_qk_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch
         dq_out = dq_out.contiguous()
     if dk_out.stride(-1) != 1:
         dk_out = dk_out.contiguous()
-    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
-    dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+    dq, dk = _new(q), _new(k)
+    dqw = None if q_weight is None else _new(q_weight)
+    dkw = None if k_weight is None else _new(k_weight)
     lib, c = load(), ctx(dev)
     ws = _Workspace.get(dev, lib.xfold_qk_norm_rotate_bwd_workspace_bytes(c, n[4]))
     desc = QK_NORM.pack(*n, *_heads(dq, ""), *_heads(dk, ""), *_heads(dq_out, ""), *_heads(dk_out, ""))
