@@ -28,6 +28,23 @@ __device__ __forceinline__ int quantise(float x, float s, float r) {
   return int(q);
 }
 
+// A row's scale by the bits of its largest magnitude, its reciprocal in two parts, and how near to a half a remainder is taken
+// for one.
+struct RowScale {
+  float s, r, r_low, near;
+  bool some;
+  __device__ __forceinline__ explicit RowScale(uint32_t most) {
+    s = __uint_as_float(most) / 127.f;
+    const bool fine = most < 0x7f800000u;
+    some = fine && s >= FLT_MIN;
+    if (!some) s = fine ? 0.f : __uint_as_float(0x7fffffffu);
+    r = some ? 1.f / s : 0.f;
+    const bool low = some && s < 1e20f;  // (r_low of larger scales would be subnormal)
+    r_low = low ? fmaf(-r, s, 1.f) * r : 0.f;
+    near = low ? 1.2e-7f : 1e-4f;
+  }
+};
+
 struct QuantArgs {
   const void* x;
   long long ldx, M, ldq;
@@ -172,13 +189,8 @@ __global__ void __launch_bounds__(1024) quantise_rows_kernel(const QuantArgs a) 
     for (int w = 0; w < tpr / 32; ++w) most = max(most, part[w0 + w]);
   }
   if (!in) return;
-  float s = __uint_as_float(most) / 127.f, r;
-  const bool fine = most < 0x7f800000u, some = fine && s >= FLT_MIN;
-  if (!some) s = fine ? 0.f : __uint_as_float(0x7fffffffu);
-  r = some ? 1.f / s : 0.f;
-  const bool low = some && s < 1e20f;  // (r_low of larger scales would be subnormal)
-  const float r_low = low ? fmaf(-r, s, 1.f) * r : 0.f, near = low ? 1.2e-7f : 1e-4f;
-  if (t == 0) a.scale[m] = s;
+  const RowScale r(most);
+  if (t == 0) a.scale[m] = r.s;
   int8_t* q = a.q + m * a.ldq;
   auto put = [&](uint2 w, int i) {
     if (a.wide_q) {
@@ -190,11 +202,11 @@ __global__ void __launch_bounds__(1024) quantise_rows_kernel(const QuantArgs a) 
   if constexpr (HELD) {
 #pragma unroll
     for (int i = 0; i < QUANT_PIECES<T>; ++i)
-      if (t + i * tpr < pieces) put(some ? p[i].quantised(s, r, r_low, near) : make_uint2(0, 0), t + i * tpr);
+      if (t + i * tpr < pieces) put(r.some ? p[i].quantised(r.s, r.r, r.r_low, r.near) : make_uint2(0, 0), t + i * tpr);
   } else {
     for (int i = t; i < pieces; i += tpr) {
       p[0].load(a, x, i, a.K - i * 8);
-      put(some ? p[0].quantised(s, r, r_low, near) : make_uint2(0, 0), i);
+      put(r.some ? p[0].quantised(r.s, r.r, r.r_low, r.near) : make_uint2(0, 0), i);
     }
   }
   for (int i = pieces + t; i * 8 < a.pitch; i += tpr) put(make_uint2(0, 0), i);
@@ -510,6 +522,146 @@ static int launch_i8(Ctx* c, const int8_t* x, long long ldx, const float* x_scal
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows (a decoding step): bound by the weights, which are read once, 16 bytes to a lane, two channels to a warp, straight
+// into the dot products of four bytes.  With one or two rows every CTA quantises them for itself while its weights are on their
+// way, and the whole layer is one launch.  (4096 x 4096, weights from memory: one row 6.1 us, by quantise_rows_kernel and the
+// tensor cores' tiles, of which there are but 64, 13.4; four rows, quantised before, 6.6 against 12.1; of eight rows the dot products take as long as the tiles.)
+// ---------------------------------------------------------------------------------------------
+constexpr int ROWS_MOST = 4, ROWS_SMEM = 48 * 1024 - 1024;  // rows; bytes of quantised rows in shared memory
+constexpr int ROWS_C = 2, ROWS_U = 4;                       // channels of a warp; pieces of each that a lane has on their way
+
+struct RowsArgs {
+  QuantArgs x;            // (quantised rows: x, ldx, M, K, and the scales)
+  const int8_t* w;
+  long long ldw;
+  int N;
+  const float *w_scale, *bias;
+  void* out;
+  long long ldo;
+  int out_f32;
+};
+
+// 16 bytes of a row of K; what lies behind it is zero, and not read
+__device__ __forceinline__ uint4 sixteen(const int8_t* row, int piece, int K) {
+  const int8_t* at = row + (long long)piece * 16;
+  if (piece * 16 + 16 <= K) return *reinterpret_cast<const uint4*>(at);
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (piece * 16 + e < K) v[e / 4] |= uint32_t(uint8_t(at[e])) << (e % 4 * 8);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <typename T, int MB>
+__global__ void __launch_bounds__(256) i8_rows_kernel(const RowsArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ float scale[MB];
+  __shared__ uint32_t part[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, K = a.x.K, pieces = (K + 15) / 16, M = (int)a.x.M;
+  const int n0 = (blockIdx.x * 8 + warp) * ROWS_C;
+  pdl_wait();
+  pdl_launch();
+  uint4 w[ROWS_C][ROWS_U];
+  auto load = [&](int u, int piece) {
+#pragma unroll
+    for (int c = 0; c < ROWS_C; ++c) {
+      w[c][u] = make_uint4(0, 0, 0, 0);
+      if (n0 + c < a.N && piece < pieces) w[c][u] = sixteen(a.w + (n0 + c) * a.ldw, piece, K);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < ROWS_U; ++u) load(u, u * 32 + lane);
+
+  // the rows in 8 bits, 256 / MB threads to each
+  constexpr int TPR = 256 / MB;
+  const int m = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  int8_t* q = reinterpret_cast<int8_t*>(smem_raw) + (size_t)m * pieces * 16;
+  if constexpr (sizeof(T) == 1) {
+    const int8_t* row = static_cast<const int8_t*>(a.x.x) + m * a.x.ldx;
+    for (int i = t; i < pieces; i += TPR)
+      reinterpret_cast<uint4*>(q)[i] = m < M ? sixteen(row, i, K) : make_uint4(0, 0, 0, 0);
+    if (t == 0) scale[m] = m < M ? a.x.scale[m] : 0.f;
+  } else {
+    const T* row = static_cast<const T*>(a.x.x) + m * a.x.ldx;
+    const int eights = m < M ? (K + 7) / 8 : 0;
+    Eight<T, false> p;
+    uint32_t most = 0;
+    for (int i = t; i < eights; i += TPR) {
+      p.load(a.x, row, i, K - i * 8);
+      p.most(most);
+    }
+    if (sizeof(T) == 2) most = max(most & 0xffffu, most >> 16) << 16;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) part[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TPR / 32; ++k) most = max(most, part[m * (TPR / 32) + k]);
+    const RowScale r(most);
+    if (t == 0) scale[m] = r.s;
+    for (int i = t; i < pieces * 2; i += TPR) {
+      uint2 v = make_uint2(0, 0);
+      if (i < eights && r.some) {
+        p.load(a.x, row, i, K - i * 8);
+        v = p.quantised(r.s, r.r, r.r_low, r.near);
+      }
+      reinterpret_cast<uint2*>(q)[i] = v;
+    }
+  }
+  __syncthreads();
+
+  int sum[ROWS_C][MB] = {};
+  for (int base = 0; base < pieces; base += 32 * ROWS_U) {
+#pragma unroll
+    for (int u = 0; u < ROWS_U; ++u) {
+      const int piece = base + u * 32 + lane;
+      if (piece < pieces) {
+#pragma unroll
+        for (int r = 0; r < MB; ++r) {
+          const int4 x = reinterpret_cast<const int4*>(smem_raw)[r * pieces + piece];
+#pragma unroll
+          for (int c = 0; c < ROWS_C; ++c) {
+            int d = __dp4a(x.x, int(w[c][u].x), sum[c][r]);
+            d = __dp4a(x.y, int(w[c][u].y), d);
+            d = __dp4a(x.z, int(w[c][u].z), d);
+            sum[c][r] = __dp4a(x.w, int(w[c][u].w), d);
+          }
+        }
+      }
+      load(u, piece + 32 * ROWS_U);
+    }
+  }
+  int mine = 0;  // lane c * MB + r: row r of channel c
+#pragma unroll
+  for (int c = 0; c < ROWS_C; ++c)
+#pragma unroll
+    for (int r = 0; r < MB; ++r) {
+      const int all = __reduce_add_sync(0xffffffffu, sum[c][r]);
+      if (lane == c * MB + r) mine = all;
+    }
+  const int n = n0 + lane / MB, r = lane % MB;
+  if (lane < ROWS_C * MB && n < a.N && r < M) {
+    const float y = fmaf(float(mine), scale[r] * a.w_scale[n], a.bias ? a.bias[n] : 0.f);
+    if (a.out_f32) static_cast<float*>(a.out)[r * a.ldo + n] = y;
+    else static_cast<bf16*>(a.out)[r * a.ldo + n] = __float2bfloat16(y);
+  }
+}
+
+static int rows_bound(long long M) { return M <= 1 ? 1 : M <= 2 ? 2 : 4; }
+static bool i8_few_rows(long long M, int K) { return M <= ROWS_MOST && rows_bound(M) * ((K + 15ll) / 16 * 16) <= ROWS_SMEM; }
+// beyond this a CTA takes longer to quantise the rows than a launch costs (2 x 4096: 7.6 us, by two launches 7.8; 4 x 4096: 12.5
+// and 9)
+static bool i8_one_launch(long long M, int K) { return i8_few_rows(M, K) && (long long)rows_bound(M) * K <= 8192; }
+
+template <typename T>
+static int launch_i8_rows(Ctx* c, const RowsArgs& a, cudaStream_t st) {
+  const int mb = rows_bound(a.x.M);
+  auto kern = mb == 1 ? i8_rows_kernel<T, 1> : mb == 2 ? i8_rows_kernel<T, 2> : i8_rows_kernel<T, 4>;
+  ProfScope ps(c, XFOLD_K_LINEAR, st);
+  launch_pdl(kern, dim3((a.N + 8 * ROWS_C - 1) / (8 * ROWS_C)), 256, (size_t)mb * ((a.x.K + 15) / 16 * 16), st, a);
+  return check_launch(c, "i8_rows_kernel");
+}
+
 static int i8_check(Ctx* c, long long M, int K, int N) {
   if (M < 0 || K < 1 || N < 0) return fail(c, XFOLD_ERR_ARG, "int8 linear: sizes");
   // 127 * 127 * K stays within the 32-bit sums
@@ -530,6 +682,8 @@ static int i8_product(Ctx* c, const int8_t* x, long long ldx, const float* x_sca
   if (!x_scale || !w_scale || !out || ldo < N || (uintptr_t)out % (out_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "int8 linear: scales and result");
   if (int rc = i8_operand(c, x, ldx, K, "activations")) return rc;
   if (int rc = i8_operand(c, w, ldw, K, "weights")) return rc;
+  if (i8_few_rows(M, K))
+    return launch_i8_rows<int8_t>(c, {{x, ldx, M, 0, nullptr, const_cast<float*>(x_scale), K, 0, 0, 0}, w, ldw, N, w_scale, bias, out, ldo, out_f32}, st);
   return out_f32 ? launch_i8(c, x, ldx, x_scale, M, K, w, ldw, N, w_scale, bias, (float*)out, ldo, early_b, st)
                  : launch_i8(c, x, ldx, x_scale, M, K, w, ldw, N, w_scale, bias, (bf16*)out, ldo, early_b, st);
 }
@@ -572,7 +726,7 @@ int xfold_linear_int8_quantized_fwd(xfold_ctx* cx, const void* x, long long ldx,
 }
 
 size_t xfold_linear_int8_workspace_bytes(long long M, int K) {
-  return M > 0 && K > 0 ? align_up((size_t)M * pad64(K), 1024) + align_up((size_t)M * 4, 1024) + 1024 : 0;
+  return M > 0 && K > 0 && !i8_one_launch(M, K) ? align_up((size_t)M * pad64(K), 1024) + align_up((size_t)M * 4, 1024) + 1024 : 0;
 }
 
 int xfold_linear_int8_fwd(xfold_ctx* cx, const void* x, int is_f32, long long ldx, long long M, int K, const void* w, long long ldw, int N,
@@ -585,15 +739,20 @@ int xfold_linear_int8_fwd(xfold_ctx* cx, const void* x, int is_f32, long long ld
   if (!M || !N) return XFOLD_OK;
   if (is_f32 != 0 && is_f32 != 1) return fail(c, XFOLD_ERR_ARG, "int8 linear: type");
   if (!x || ldx < K || (uintptr_t)x % (is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "int8 linear: null or misaligned activations");
-  Carver cv(ws, ws_bytes);
-  int8_t* q = (int8_t*)cv.take((size_t)M * pad64(K));
-  float* scale = (float*)cv.take((size_t)M * 4);
-  if (!ws || (uintptr_t)ws % 16 || !cv.ok()) return fail(c, XFOLD_ERR_ARG, "int8 linear: workspace too small (%zu < %zu) or misaligned", ws_bytes, cv.off);
   // what the product would refuse is refused before the first launch
+  if (out_is_f32 != 0 && out_is_f32 != 1) return fail(c, XFOLD_ERR_ARG, "int8 linear: type of the result");
   if (int rc = i8_operand(c, w, ldw, K, "weights")) return rc;
   if (!w_scale || !out || ldo < N || (uintptr_t)out % (out_is_f32 ? 4 : 2)) return fail(c, XFOLD_ERR_ARG, "int8 linear: scales and result");
   DeviceGuard dev(c);
   cudaStream_t st = (cudaStream_t)stream;
+  if (i8_one_launch(M, K)) {
+    const RowsArgs a{{x, ldx, M, 0, nullptr, nullptr, K, 0, 0, 0}, (const int8_t*)w, ldw, N, w_scale, bias, out, ldo, out_is_f32};
+    return is_f32 ? launch_i8_rows<float>(c, a, st) : launch_i8_rows<bf16>(c, a, st);
+  }
+  Carver cv(ws, ws_bytes);
+  int8_t* q = (int8_t*)cv.take((size_t)M * pad64(K));
+  float* scale = (float*)cv.take((size_t)M * 4);
+  if (!ws || (uintptr_t)ws % 16 || !cv.ok()) return fail(c, XFOLD_ERR_ARG, "int8 linear: workspace too small (%zu < %zu) or misaligned", ws_bytes, cv.off);
   if (int rc = launch_quantise(c, x, is_f32, ldx, M, K, q, pad64(K), (int)pad16(K), scale, st)) return rc;
   // the quantisation starts behind what wrote the weights, and the product is launched behind its start
   return i8_product(c, q, pad64(K), scale, M, K, (const int8_t*)w, ldw, N, w_scale, bias, out, out_is_f32, ldo, 1, st);

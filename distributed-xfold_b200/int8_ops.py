@@ -80,9 +80,10 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: O
         _refuse("int8 linear: bfloat16 or float32")
     dev, lib = _device(x, w, w_scale, bias), load()
     out = x.new_empty((m, n) if x2 is x else (*x.shape[:-1], n), dtype=dtype)
-    ws = _Workspace.get(dev, lib.xfold_linear_int8_workspace_bytes(m, k))
+    need = lib.xfold_linear_int8_workspace_bytes(m, k)   # (a row or two: none)
+    ws = _Workspace.get(dev, need) if need else None
     rc = lib.xfold_linear_int8_fwd(ctx(dev), x2.data_ptr(), xt is F32, _ld(x2), m, k, at, ldw, n, w_scale.data_ptr(), _ptr(bias),
-                                   out.data_ptr(), dtype is F32, n, ws.data_ptr(), ws.numel(), _stream(dev))
+                                   out.data_ptr(), dtype is F32, n, _ptr(ws), need, _stream(dev))
     check(rc, dev, "xfold_linear_int8_fwd")
     return out
 

@@ -219,7 +219,8 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     """Root-mean-square norm of each head of q and k, times its weight (float32 [width], None: ones) and for q ``q_scale``, then
     the rotation by position, in one pass.  q and k: bfloat16 or float32 [batch, tokens, heads, width] or without the batch, widths
     even up to 256, with as many heads each as they like and any strides between them (views of a fused projection).  positions
-    int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, which may be the inputs."""
+    int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, each of which may be
+    its own input (the same view of it)."""
     dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
     if out is None:
         qo, ko = _new(q), _new(k)
@@ -228,6 +229,10 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         for o, x in ((qo, q), (ko, k)):
             if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
                 _refuse("results of queries and keys: shape, type and device of their inputs")
+            if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
+                _refuse("results of queries and keys: one place for each element")
+        if qo.numel() and ko.numel() and (qo.data_ptr() in (ko.data_ptr(), k.data_ptr()) or ko.data_ptr() == q.data_ptr()):
+            _refuse("results of queries and keys: new, or each over its own input")
     rc = load().xfold_qk_norm_rotate_fwd(ctx(dev), QK_NORM.pack(*n, *_heads(qo, "result of the queries"), *_heads(ko, "result of the keys"),
                                                                 0, 0, 0, 0, 0, 0, 0, 0), _stream(dev))
     check(rc, dev, "xfold_qk_norm_rotate_fwd")

@@ -307,7 +307,7 @@ int xfold_quantize_rows_fwd(xfold_ctx* ctx, const void* x, int is_f32, long long
 int xfold_linear_int8_quantized_fwd(xfold_ctx* ctx, const void* x, long long ldx, const float* x_scale, long long M, int K,
                                     const void* w, long long ldw, int N, const float* w_scale, const float* bias, void* out,
                                     int out_is_f32, long long ldo, void* stream);
-/* Both in one call, x bf16 or float32. */
+/* Both in one call, x bf16 or float32.  (Few rows may need no workspace: 0 bytes, ws NULL.) */
 size_t xfold_linear_int8_workspace_bytes(long long M, int K);
 int xfold_linear_int8_fwd(xfold_ctx* ctx, const void* x, int is_f32, long long ldx, long long M, int K, const void* w, long long ldw,
                           int N, const float* w_scale, const float* bias, void* out, int out_is_f32, long long ldo, void* ws,

@@ -239,3 +239,69 @@ def _attention_state(g, c):
     st = {n + ".weight": torch.randn(c, c, generator=g) * c ** -0.5 for n in ("q_projection", "k_projection", "v_projection", "gating_query")}
     st["adaptive_zero_init.transition2.weight"] = torch.randn(c, c, generator=g) * c ** -0.5
     return st
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_rows_that_start_anywhere(Q, dtype):
+    """Rows at any element of an array that ends with them, widths on both sides of eight and sixteen; whole and apart."""
+    g = gen(31)
+    for k in (1, 7, 8, 9, 15, 16, 17, 31, 40, 250):
+        for off in range(8):
+            flat = torch.randn(off + 5 * k, generator=g).to(dtype).cuda()
+            views = [flat[off:].view(5, k)]
+            if k > off:
+                views.append(torch.randn(5, k, generator=g).to(dtype).cuda()[:, off:])
+            for x in views:
+                want, scale = plain_rows(x.cpu())
+                q, s = Q.quantize_rows(x)
+                assert torch.equal(s.cpu(), scale) and torch.equal(q.cpu().double(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [1.0, 3.7e-5, 1e-30, 1e19, 3e22, 1e36])
+def test_quantize_rows_near_to_halves(Q, dtype, scale):
+    """Quotients at and next to a half, as 16-bit numbers have many: whole numbers and halves, their largest 127 or anything."""
+    g = gen(17)
+    x = (torch.randn(300, 1001, generator=g) * 40).clamp(-126, 126)
+    for t in (x.round() + 0.5, x.round(), x):
+        for first in (127.0, 126.0, None):
+            y = t.clone()
+            if first is not None:
+                y[:, 0] = first
+            y = (y * scale).to(dtype)
+            want, s64 = plain_rows(y)
+            q, s = Q.quantize_rows(y.cuda())
+            assert torch.equal(s.cpu(), s64) and torch.equal(q.cpu().double(), want)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("k,n", [(1, 3), (15, 1), (17, 40), (1000, 37), (2048, 100), (4096, 64), (4100, 33), (9000, 20), (50000, 9)])
+def test_linear_int8_of_few_rows(Q, ops, m, k, n):
+    """A decoding step: the same bits whether the rows are quantised in the call, before it, or among many rows."""
+    g = gen(m * k + n)
+    x = torch.randn(m, k, generator=g).to(BF).cuda()
+    w, ws = weights(n, k, 5)
+    bias = torch.randn(n, generator=g).cuda()
+    out = Q.linear_int8(x, w, ws, bias)
+    q, s = plain_rows(x.cpu())
+    check_linear(out, q, s, w, ws, bias, BF)
+    xq, xs = Q.quantize_rows(x)
+    assert torch.equal(Q.linear_int8_quantized(xq, xs, w, ws, bias, BF), out)
+    many = torch.cat([x, torch.ones(130, k, dtype=BF, device="cuda")])
+    assert torch.equal(Q.linear_int8(many, w, ws, bias)[:m], out)
+    f = Q.linear_int8(x.float(), w, ws, None, dtype=F32)
+    check_linear(f, *plain_rows(x.float().cpu()), w, ws, None, F32)
+    ops.synchronize_and_check()
+
+
+def test_linear_int8_does_not_read_behind_the_last_row(Q):
+    """Weights whose last row ends with the array, at widths that are no multiple of 16; rows of x that hold nothing finite."""
+    for k in (1, 33, 1000, 1023):
+        pitch = (k + 15) // 16 * 16
+        flat = torch.full((4 * pitch + k,), 3, dtype=I8, device="cuda")
+        w = torch.as_strided(flat, (5, k), (pitch, 1))
+        x = torch.ones(3, k, dtype=F32, device="cuda")
+        x[1, k // 2] = float("inf")
+        out = Q.linear_int8(x, w, torch.ones(5).cuda())
+        assert out[1].isnan().all() and torch.equal(out[0], out[2])
+        assert float((out[0].double() - 3.0 * k).abs().max()) <= 3.0 * k * 4 * U

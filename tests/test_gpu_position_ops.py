@@ -444,3 +444,71 @@ def test_position_calls_captured(P, ops):
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want[seed]))
     del filler
+
+
+def test_norm_rotate_results_that_are_refused(P):
+    from distributed_xfold_b200._cabi import XfoldError
+    q, k = torch.randn(3, 4, 8).cuda(), torch.randn(3, 4, 8).cuda()
+    for out in ((k, q), (k, torch.empty_like(k)), (q, q), (q[:1].expand(3, -1, -1), k), (q[..., :4], k), (q, k.to(BF))):
+        with pytest.raises(XfoldError, match="results of queries and keys"):
+            P.norm_rotate_qk(q, k, None, None, out=out)
+
+
+RANGES = [  # batch, tokens, q heads, k heads, width, rotated, interleaved, type: warps whose passes begin and end inside tokens
+    (3, 700, 12, 4, 128, 128, False, BF),
+    (2, 1300, 16, 16, 64, 32, True, BF),
+    (1, 5000, 5, 0, 48, 48, False, F32),
+    (5, 401, 0, 9, 80, 40, True, BF),
+    (2, 900, 33, 1, 256, 256, True, BF),
+]
+
+
+@pytest.mark.parametrize("case", RANGES)
+def test_norm_rotate_of_many_tokens(P, ops, case):
+    """Positions on both sides of zero; every token against the definition, forward and backward."""
+    b, s, hq, hk, d, rot, inter, dtype = case
+    q, k, qw, kw, rotation, pos = qk_case(P, b, s, hq, hk, d, rot, inter, dtype, -20, seed=3)
+    pos = pos * torch.tensor([1, -1000003])[torch.arange(s) % 2].int()
+    check_forward(P, q, k, qw, kw, rotation, pos, pos, 1e-6, 0.25, P.norm_rotate_qk(q, k, qw, kw, rotation, pos.cuda(), q_scale=0.25)) \
+        if hq and hk else None
+    g = gen(s)
+    dq, dk = (torch.randn(x.shape, generator=g).to(dtype).cuda() for x in (q, k))
+    got = P.norm_rotate_qk_backward(dq, dk, q, k, qw, kw, rotation, pos.cuda(), q_scale=0.25)
+    for x, dy, w, f, dx, dw in ((q, dq, qw, 0.25, got[0], got[2]), (k, dk, kw, 1.0, got[1], got[3])):
+        if not x.numel():
+            assert not dw.any()
+            continue
+        x64, w64, d64 = x.double().cpu(), w.double().cpu(), dy.double().cpu()
+        back, size = turned(d64, rotation, pos, back=True) * f, pair_length(d64, rotation) * f
+        r = (x64.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        want = r * (back * w64 - x64 * r * r * (back * w64 * x64).mean(-1, keepdim=True))
+        tol = 96 * U * r * (size * w64.abs() + x64.abs() * r * r * (size * (w64 * x64).abs()).mean(-1, keepdim=True))
+        tol = tol + HALF[dtype] * (want.abs() + tol) + 2.0 ** -133
+        assert ((dx.double().cpu() - want).abs() <= tol).all()
+        want, most = (back * x64 * r).sum((0, 1, 2)), (size * x64.abs() * r).sum((0, 1, 2))
+        # a lane's chain, the lanes of a warp, four warps, the CTAs in 32 chains: far fewer additions than heads and tokens
+        assert ((dw.double().cpu() - want).abs() <= (x[..., 0].numel() / 16 + 512) * U * most).all()
+    ops.synchronize_and_check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("sq,sk,heads,groups,reach", [(1, 700, 3, 2, 5), (9, 8, 2, 0, 0), (1000, 264, 16, 3, 0), (257, 1000, 40, 7, 64), (2050, 96, 2, 0, 700)])
+def test_relative_bias_gradient_of_eights(P, ops, dtype, sq, sk, heads, groups, reach):
+    """Rows in eights that end anywhere, groups and positions that change inside an eight; whole numbers: equal."""
+    g = gen(sq + reach)
+    qp, kp = (torch.randint(-400, 400, (n,), generator=g).int().sort().values for n in (sq, sk))
+    qp[::5] = qp[torch.randint(0, sq, (len(qp[::5]),), generator=g)]
+    qg, kg = (torch.randint(0, groups, (n,), generator=g).int().sort().values if groups else None for n in (sq, sk))
+    nb = 2 * reach + 1 + bool(groups)
+    b = (kp.long()[None] - qp.long()[:, None]).clamp(-reach, reach) + reach
+    if groups:
+        b = torch.where(qg[:, None] == kg[None], b, nb - 1)
+    if nb > 1024:
+        b = b.clamp(max=1023)
+    grad = torch.randint(-4, 5, (heads, sq, sk), generator=g).to(dtype)
+    lut = torch.arange(2 * reach + 1, dtype=torch.int32).clamp(max=1023)
+    cu = lambda t: None if t is None else t.cuda()
+    got = P.relative_position_bias_backward(grad.cuda(), min(nb, 1024), lut.cuda(), cu(qp), cu(kp), cu(qg), cu(kg))
+    want = torch.zeros(heads, min(nb, 1024), dtype=F64).index_add_(1, b.flatten(), grad.flatten(1).double()).T
+    assert torch.equal(got.double().cpu(), want)
+    ops.synchronize_and_check()
