@@ -65,33 +65,42 @@ struct alignas(sizeof(E) * V) RelPiece {
 };
 
 // A thread keeps V columns and goes down the rows: their positions stay in registers, and a row's buckets serve all heads of
-// the CTA.  Where the V columns share a bucket (beyond the reach, or in another group) a head's value is fetched once.
+// the CTA.  Where the V columns share a bucket (beyond the reach, or in another group), and those of the warp's other lanes do
+// too, a head's value is fetched once.  Bound by the result's bytes, in the order that CTAs come by them: 16 heads x 2048^2
+// float32 44 us (a fill with zeros 37), 16 bits 26, prepared 16 x 1999 x 2000 23.  Rows of odd lengths as plain numbers are
+// written element by element (16 x 1999^2 float32 67, 16 bits 47).
 template <typename E, int V>
-__global__ void __launch_bounds__(256) rel_bias_kernel(const RelFwdArgs a) {
+__global__ void __launch_bounds__(256, V == 1 ? 4 : 1) rel_bias_kernel(const RelFwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   const RelShared& s = a.s;
   const int rows_tab = s.nb + 2, h0 = blockIdx.z * a.hg, hn = min(a.hg, s.H - h0);
   E* tab = reinterpret_cast<E*>(smem_raw);  // [hg][nb + 2]: row nb is zero, row nb + 1 not a number
   uint16_t* lut = reinterpret_cast<uint16_t*>(smem_raw + (((size_t)a.hg * rows_tab * sizeof(E) + 15) & ~size_t(15)));
-  pdl_wait();
-  pdl_launch();
-  stage_lut(s, lut);
-  for (int i = threadIdx.x; i < hn * rows_tab; i += 256) {
-    const int h = i / rows_tab, b = i % rows_tab;
-    rel_value(b < s.nb ? a.table[(long long)b * s.H + h0 + h] : b == s.nb ? 0.f : __int_as_float(0x7fffffff), tab[i]);
-  }
-  __syncthreads();
   const int cx = 1 << a.log_cx, ry = 256 >> a.log_cx;
   const long long col = ((long long)blockIdx.x * cx + (threadIdx.x & (cx - 1))) * V;
-  if (col >= a.cols) return;
-  int kp[V], kg[V], pmin = 0x7fffffff, pmax = -0x7fffffff - 1;
-  bool whole = true;  // one group, no padding
+  pdl_wait();
+  pdl_launch();
+  // the columns' positions are on their way while the table is made
+  int kp[V], kg[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const bool in = col + v < s.Sk;
     kp[v] = in ? s.k_pos[col + v] : 0;
     kg[v] = in && s.k_grp ? s.k_grp[col + v] : 0;
-    whole = whole && in && kg[v] == kg[0];
+  }
+  stage_lut(s, lut);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < hn * rows_tab; i += 256) {
+    const int b = i / hn, h = i - b * hn;
+    rel_value(b < s.nb ? a.table[(long long)b * s.H + h0 + h] : b == s.nb ? 0.f : __int_as_float(0x7fffffff), tab[h * rows_tab + b]);
+  }
+  __syncthreads();
+  if (col >= a.cols) return;
+  int pmin = 0x7fffffff, pmax = -0x7fffffff - 1;
+  bool whole = true;  // one group, no padding
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    whole = whole && col + v < s.Sk && kg[v] == kg[0];
     pmin = min(pmin, kp[v]);
     pmax = max(pmax, kp[v]);
   }
@@ -101,7 +110,8 @@ __global__ void __launch_bounds__(256) rel_bias_kernel(const RelFwdArgs a) {
     const long long plane = (long long)s.Sq * a.pitch;
     const int lo = offset_in_lut(pmin, qp, s.reach), hi = offset_in_lut(pmax, qp, s.reach);
     const bool other = whole && kg[0] != qg;
-    if (other || (whole && lo == hi)) {
+    const bool alike = other || (whole && lo == hi);
+    if (__all_sync(__activemask(), alike)) {  // (whichever lanes are together: a warp goes one way, not both)
       const E* t = tab + (other ? s.nb - 1 : int(lut[lo]));
 #pragma unroll 4
       for (int h = 0; h < hn; ++h, t += rows_tab, dst += plane) {
