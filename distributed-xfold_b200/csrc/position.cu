@@ -70,7 +70,7 @@ struct alignas(sizeof(E) * V) RelPiece {
 // float32 44 us (a fill with zeros 37), 16 bits 26, prepared 16 x 1999 x 2000 23.  Rows of odd lengths as plain numbers are
 // written element by element (16 x 1999^2 float32 67, 16 bits 47).
 template <typename E, int V>
-__global__ void __launch_bounds__(256, V == 1 ? 4 : 1) rel_bias_kernel(const RelFwdArgs a) {
+__global__ void __launch_bounds__(256, V == 1 ? 4 : 0) rel_bias_kernel(const RelFwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   const RelShared& s = a.s;
   const int rows_tab = s.nb + 2, h0 = blockIdx.z * a.hg, hn = min(a.hg, s.H - h0);
