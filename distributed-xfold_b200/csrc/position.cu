@@ -163,6 +163,9 @@ static void launch_rel_fwd(Ctx* c, RelFwdArgs a, cudaStream_t st) {
 // atomics, and the order of the sum is always the same).
 // The eights of a CTA lie `slices` apart, so that every warp has its share of the band.  CTAs leave their sums in the workspace;
 // a second kernel adds them.
+// 16 heads x 2048^2 in 16 bits, buckets up to 128 apart: 33.6 us for both (4.0 TB/s; without a band 24.3, the bytes 20.5), float32
+// 47.5 (5.6 TB/s).  Row by row instead of by eights 45: two dozen instructions for each row and block of columns to find out
+// where it lies.  Bound by the band's reads and writes of shared memory, then by bytes; small ones by the two launches.
 // ---------------------------------------------------------------------------------------------
 struct RelBwdArgs {
   RelShared s;
@@ -426,8 +429,14 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
 // G lanes share a head; a lane holds two pieces of V elements that rotate into each other: of the halves, or 2 V neighbours
 // (beyond `rot`: 2 V neighbours that do not rotate).  Its place in the head is the same for all heads of a token, and so an
 // element of the result is own * A + partner * B (and r, the reciprocal root), with A and B made of weights, cosines and sines
-// once for a token: in registers, at three instructions for two elements.  Angles are made once for a token and warp, in turns
-// and in 64 bits until the whole turns are gone: 32 bits would lose far positions.
+// once for a token: in registers, at three instructions for two elements.  Angles are made once for a token and warp, as 64-bit
+// fractions of a turn: 32-bit floats would lose far positions.
+// Pieces are 16 bytes where sizes allow it: of 8, sums over twice as many lanes and addresses for half as much work cost more than
+// the fewer registers give back (4 x 4096 tokens, 32 + 8 heads of 128 in 16 bits: 79 and, backward, 137 us).  Warps take ranges of
+// passes that begin and end anywhere in a token, so that none has a token more than another.
+// Now 62 us (5.4 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64: 9.4 and 17.9.  Bound by bytes and the chain of a pass
+// (sums over the lanes, root); where a head's width is no power of two some lanes idle (80 of 128: 5 of 8 lanes; groups of any
+// size were slower, by their sums).
 // ---------------------------------------------------------------------------------------------
 struct QkTensor {
   const void *x, *d;  // d: gradient of the result (backward)
