@@ -528,20 +528,25 @@ __device__ __forceinline__ QkPlace qk_place(const QkArgs& a, int sl) {
 }
 
 // An angle's whole turns are of no interest, so turns for each position are kept as a fraction of 64 bits (once for a CTA), and
-// their product with the position as one that wraps around: exact but for the fraction's last bit, times the position.
+// their product with the position as one that wraps around: exact but for the fraction's last bit, times the position.  The lowest
+// of them stands for a frequency that is not finite (of half a turn the next is as good).
+constexpr unsigned long long NO_ANGLE = 1ull << 63;
 __device__ __forceinline__ void qk_turns_of_a_position(const QkArgs& a, unsigned long long* turns) {
   for (int i = threadIdx.x; i < a.rot / 2; i += blockDim.x) {
     const double f = a.freqs[i] * 0.15915494309189533577;  // 1 / (2 pi)
-    turns[i] = (unsigned long long)__double2ll_rn((f - rint(f)) * 18446744073709551616.0);
+    const long long part = __double2ll_rn((f - rint(f)) * 18446744073709551616.0);
+    turns[i] = !isfinite(f) ? NO_ANGLE : (unsigned long long)part == NO_ANGLE ? NO_ANGLE + 1 : (unsigned long long)part;
   }
 }
 // cosines and sines of a position's angles, by a warp
 __device__ __forceinline__ void qk_angles(const QkArgs& a, const unsigned long long* turns, int pos, float2* sm) {
   __syncwarp();
   for (int i = threadIdx.x & 31; i < a.rot / 2; i += 32) {
-    const int part = int((turns[i] * (unsigned long long)(long long)pos) >> 32);  // of 2^32
+    const unsigned long long turn = turns[i];
+    const int part = int((turn * (unsigned long long)(long long)pos) >> 32);  // of 2^32
     float c, s;
     sincospif(float(part) * 0x1p-31f, &s, &c);
+    if (turn == NO_ANGLE) c = s = __int_as_float(0x7fffffff);
     sm[i] = make_float2(c, s);
   }
   __syncwarp();

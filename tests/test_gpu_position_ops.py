@@ -512,3 +512,21 @@ def test_relative_bias_gradient_of_eights(P, ops, dtype, sq, sk, heads, groups, 
     want = torch.zeros(heads, min(nb, 1024), dtype=F64).index_add_(1, b.flatten(), grad.flatten(1).double()).T
     assert torch.equal(got.double().cpu(), want)
     ops.synchronize_and_check()
+
+
+def test_norm_rotate_of_odd_frequencies(P):
+    """Whole and half turns for each position, many turns, and frequencies that are not finite: those pairs are not numbers."""
+    f = torch.tensor([math.pi, 2 * math.pi, 3 * math.pi, 1e5, -0.3, 0.0, float("nan"), float("inf")], dtype=F64)
+    q = torch.randn(1, 9, 2, 16, generator=gen(4)).cuda()
+    pos = torch.tensor([[0, 1, 2, 3, -1, 7, 1000001, -2 ** 31, 2 ** 31 - 1]]).int()
+    finite = P.Rotation(f[:6])
+    keep = torch.cat([q[..., :6], q[..., 8:14]], -1).contiguous()
+    a, b = P.norm_rotate_qk(keep, keep, None, None, P.Rotation(f[:6].cuda()), pos.cuda())
+    y = plain(keep, None, None, pos, 1e-6, 1.0)
+    # the definition's own angle is a product in 64 bits: up to 2^31 * 1e5 radians, off by 2^-53 of it, beside the kernel's
+    tol = 32 * U * pair_length(y, finite) + (pos.double().abs()[..., None] * f[:6].abs() * 2.0 ** -51).repeat(1, 1, 2)[:, :, None] * pair_length(y, finite)
+    want = turned(y, finite, pos)
+    for got in (a, b):
+        assert ((got.double().cpu() - want).abs() <= tol + U * want.abs()).all()
+    a, _ = P.norm_rotate_qk(q, q, None, None, P.Rotation(f.cuda()), pos.cuda())
+    assert a[..., [6, 7, 14, 15]].isnan().all() and a[..., [0, 1, 2, 3, 4, 5, 8, 9, 10, 11, 12, 13]].isfinite().all()
