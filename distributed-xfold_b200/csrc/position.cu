@@ -67,7 +67,7 @@ struct alignas(sizeof(E) * V) RelPiece {
 // A thread keeps V columns and goes down the rows: their positions stay in registers, and a row's buckets serve all heads of
 // the CTA.  Where the V columns share a bucket (beyond the reach, or in another group), and those of the warp's other lanes do
 // too, a head's value is fetched once.  Bound by the result's bytes, in the order that CTAs come by them: 16 heads x 2048^2
-// float32 44 us (a fill with zeros 37), 16 bits 26, prepared 16 x 1999 x 2000 23.  Rows of odd lengths as plain numbers are
+// float32 44 us (a fill with zeros 37), 16 bits 24, prepared 16 x 1999 x 2000 24.  Rows of odd lengths as plain numbers are
 // written element by element (16 x 1999^2 float32 67, 16 bits 47).
 template <typename E, int V>
 __global__ void __launch_bounds__(256, V == 1 ? 4 : 0) rel_bias_kernel(const RelFwdArgs a) {
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(256, V == 1 ? 4 : 0) rel_bias_kernel(const Rel
       for (int v = 0; v < V; ++v)
         b[v] = col + v >= s.Sk ? s.nb : kg[v] != qg ? s.nb - 1 : int(lut[offset_in_lut(kp[v], qp, s.reach)]);
       const E* t = tab;
-#pragma unroll 4
+#pragma unroll(V == 8 ? 1 : 4)  // (eight reads of the table are enough on their way, and 64 registers let four CTAs on an SM)
       for (int h = 0; h < hn; ++h, t += rows_tab, dst += plane) {
         RelPiece<E, V> p;
 #pragma unroll
