@@ -18,7 +18,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     (m, k), (ld, e) = x.shape, x.stride()
-    return x if k <= 1 or (e == 1 and (ld >= k or m <= 1)) else x.contiguous()
+    return x if (e == 1 or k <= 1) and (ld >= k or m <= 1) else x.contiguous()
 
 
 def _ld(x2: torch.Tensor) -> int:

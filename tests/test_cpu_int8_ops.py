@@ -53,3 +53,15 @@ def test_refused_quantized(Q):
         Q.quantize_rows(torch.zeros(3, 4, dtype=torch.float64))
     with pytest.raises(XfoldError, match="GPU only"):
         Q.quantize_rows(torch.zeros(3, 4))
+
+
+@pytest.mark.parametrize("shape,strides", [((5, 1), (0, 1)), ((5, 1), (0, 7)), ((5, 1), (3, 9)), ((1, 1), (0, 0)), ((5, 4), (0, 1)), ((5, 4), (2, 1)), ((1, 4), (0, 1)),
+                                           ((5, 4), (8, 2)), ((5, 4), (6, 1)), ((2, 3, 1), (0, 0, 1)), ((2, 3, 4), (0, 4, 1))])
+def test_rows_of_activations_lie_in_their_memory(Q, shape, strides):
+    """Whatever the strides: the rows that a call hands on, taken one row stride apart, hold x and end where its memory ends."""
+    x = torch.as_strided(torch.randn(1 + sum((n - 1) * s for n, s in zip(shape, strides))), shape, strides)
+    rows = Q._rows(x)
+    m, k = rows.shape
+    read = rows.storage_offset() + (m - 1) * Q._ld(rows) + k
+    assert read * 4 <= rows.untyped_storage().nbytes()
+    assert torch.equal(torch.as_strided(rows, (m, k), (Q._ld(rows), 1)), x.reshape(-1, k))

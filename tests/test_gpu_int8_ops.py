@@ -305,3 +305,16 @@ def test_linear_int8_does_not_read_behind_the_last_row(Q):
         out = Q.linear_int8(x, w, torch.ones(5).cuda())
         assert out[1].isnan().all() and torch.equal(out[0], out[2])
         assert float((out[0].double() - 3.0 * k).abs().max()) <= 3.0 * k * 4 * U
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_one_number_broadcast_over_the_rows(Q, ops, dtype):
+    """Rows of one element that all are the same one, as an expanded tensor has them."""
+    x = torch.full((1, 1), -2.5, dtype=dtype).cuda()
+    w, ws = weights(20, 1, 3)
+    for m in (2, 5, 300):
+        wide = x.expand(m, 1)
+        q, s = Q.quantize_rows(wide)
+        assert (q == -127).all() and torch.equal(s, Q.quantize_rows(x)[1].expand(m))
+        assert torch.equal(Q.linear_int8(wide, w, ws), Q.linear_int8(wide.contiguous(), w, ws))
+    ops.synchronize_and_check()
