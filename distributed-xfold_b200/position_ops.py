@@ -207,6 +207,99 @@ def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x, memory_format=torch.contiguous_format)   # (half the host time of new_empty)
 
 
+def _reaches(steps, at: int) -> bool:
+    """Whether at + sum step * n can be 0, for whole numbers first <= n <= last of each (step, first, last).  Past some thousands
+    of tries: yes.  (Axes that lie within each other leave two or three tries for each.)"""
+    one = []
+    for step, first, last in sorted(steps):
+        if one and step % one[-1][0] == 0 and one[-1][2] - one[-1][1] + 1 >= step // one[-1][0]:   # together: every multiple of the shorter
+            short, a, b = one.pop()
+            step, first, last = short, a + first * (step // short), b + last * (step // short)
+        one.append((step, first, last))
+    steps = one[::-1]
+    ends = [(0, 0)]   # what the steps from each on can add
+    for step, first, last in reversed(steps):
+        ends.append((ends[-1][0] + step * first, ends[-1][1] + step * last))
+    ends.reverse()
+    tries = 4096
+
+    def find(i: int, at: int) -> bool:
+        nonlocal tries
+        tries -= 1
+        if tries < 0 or i == len(steps):
+            return tries < 0 or at == 0
+        step, first, last = steps[i]
+        down, up = ends[i + 1]
+        return any(find(i + 1, at + step * n) for n in range(max(first, -((at + up) // step)), min(last, (-at - down) // step) + 1))
+
+    return find(0, at)
+
+
+def _axes(t: torch.Tensor):
+    return [(st, n - 1) for st, n in zip(t.stride(), t.shape) if n > 1]
+
+
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of one lies where one of the other does (both of one type)."""
+    if not (a.numel() and b.numel()):
+        return False
+    (ra, rb), size = (_axes(a), _axes(b)), a.element_size()
+    at, odd = divmod(b.data_ptr() - a.data_ptr(), size)
+    if at > sum(st * n for st, n in ra) or at + 1 < -sum(st * n for st, n in rb):
+        return False
+    steps = {}
+    for st, n in rb:
+        steps[st] = (0, n) if st not in steps else (0, steps[st][1] + n)
+    for st, n in ra:
+        first, last = steps.get(st, (0, 0))
+        steps[st] = (first - n, last)
+    steps = [(st, *n) for st, n in steps.items() if st]
+    return _reaches(steps, at) or (odd > 0 and _reaches(steps, at + 1))
+
+
+def _one_place_each(t: torch.Tensor) -> bool:
+    axes, wide = sorted(_axes(t)), 1
+    for st, n in axes:
+        if st < wide:
+            break
+        wide += st * n
+    else:
+        return True
+    # not one axis within the other: two elements share a place where steps that are not all none lead nowhere
+    return not t.numel() or not any(_reaches([(st, -n, n) for st, n in axes[:i] if st] + [(axes[i][0], 1, axes[i][1])], 0) if axes[i][0] else True
+                                    for i in range(len(axes)))
+
+
+def _side_by_side(b: int, s: int, hq: int, hk: int, d: int, size: int, pq: int, qb: int, qt: int, qh: int, pk: int, kb: int, kt: int, kh: int) -> bool:
+    """Whether queries and keys by their sizes, addresses and strides are seen at once to have a place for each element: tensors one
+    behind the other, or heads side by side in the rows of one projection, as nearly all are.  (Not seen so: they may still.)"""
+    if hq < 1 or hk < 1 or b < 1 or s < 1:
+        return False
+    wq, wk = (hq - 1) * qh + d, (hk - 1) * kh + d
+    if qh < d or kh < d or (s > 1 and (qt < wq or kt < wk)) or (b > 1 and (qb < (s - 1) * qt + wq or kb < (s - 1) * kt + wk)):
+        return False
+    at = pk - pq
+    if at >= ((b - 1) * qb + (s - 1) * qt + wq) * size or -at >= ((b - 1) * kb + (s - 1) * kt + wk) * size:
+        return True
+    # (rows as long as their distance, of which both have a part)
+    return (qt == kt and (b == 1 or (qb == kb and qb >= s * qt))
+            and (wq * size <= at <= (qt - wk) * size or wk * size <= -at <= (qt - wq) * size))
+
+
+def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and _axes(a) == _axes(b)
+
+
+def _check_results(q, k, qo, ko, dev) -> None:
+    for o, x in ((qo, q), (ko, k)):
+        if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
+            _refuse("results of queries and keys: shape, type and device of their inputs")
+        if not _one_place_each(o):
+            _refuse("results of queries and keys: one place for each element")
+    if _meet(qo, ko) or _meet(qo, k) or _meet(ko, q) or any(not _same_view(o, x) and _meet(o, x) for o, x in ((qo, q), (ko, k))):
+        _refuse("results of queries and keys: new, or each over its own input")
+
+
 def _weight(w: torch.Tensor, d: int) -> int:
     if w.dtype is not F32 or w.shape != (d,) or (w.stride(0) != 1 and d > 1):
         _refuse("norm weights: float32 [width]")
@@ -220,19 +313,14 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     the rotation by position, in one pass.  q and k: bfloat16 or float32 [batch, tokens, heads, width] or without the batch, widths
     even up to 256, with as many heads each as they like and any strides between them (views of a fused projection).  positions
     int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, each of which may be
-    its own input (the same view of it)."""
+    its own input (the same view of it) and otherwise lies apart from the inputs and from the other."""
     dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
     if out is None:
         qo, ko = _new(q), _new(k)
     else:
         qo, ko = out
-        for o, x in ((qo, q), (ko, k)):
-            if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
-                _refuse("results of queries and keys: shape, type and device of their inputs")
-            if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
-                _refuse("results of queries and keys: one place for each element")
-        if qo.numel() and ko.numel() and (qo.data_ptr() in (ko.data_ptr(), k.data_ptr()) or ko.data_ptr() == q.data_ptr()):
-            _refuse("results of queries and keys: new, or each over its own input")
+        if not (qo is q and ko is k and _side_by_side(*n[:5], 4 if n[7] else 2, *n[-8:])):
+            _check_results(q, k, qo, ko, dev)
     rc = load().xfold_qk_norm_rotate_fwd(ctx(dev), QK_NORM.pack(*n, *_heads(qo, "result of the queries"), *_heads(ko, "result of the keys"),
                                                                 0, 0, 0, 0, 0, 0, 0, 0), _stream(dev))
     check(rc, dev, "xfold_qk_norm_rotate_fwd")

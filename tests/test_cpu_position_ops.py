@@ -123,3 +123,71 @@ def test_rotation_of_a_base(P):
     r = P.Rotation.make(8, base=100.0, device="cpu")
     assert r.freqs.dtype == torch.float64 and not r.interleaved
     assert torch.allclose(r.freqs, torch.tensor([1.0, 100 ** -0.25, 100 ** -0.5, 100 ** -0.75], dtype=torch.float64))
+
+
+def _places(t):
+    """Bytes of a tensor's elements."""
+    at = torch.zeros(t.shape, dtype=torch.int64)
+    for axis, (n, st) in enumerate(zip(t.shape, t.stride())):
+        at += (torch.arange(n) * st).view(-1, *[1] * (t.dim() - 1 - axis))
+    return ((at.flatten() + t.storage_offset()) * t.element_size()).tolist()
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_where_tensors_lie(P, dtype):
+    """Whether two views of one buffer meet, and whether a view has a place for each element, against all of their places."""
+    g = torch.Generator().manual_seed(7)
+    pick = lambda *n: n[int(torch.randint(0, len(n), (1,), generator=g))]
+    buf, seen, at_once = torch.zeros(200000, dtype=dtype), {}, 0
+    for _ in range(3000):
+        dims = pick(3, 4)
+        shape = [pick(1, 2, 3, 5) for _ in range(dims)]
+        views = []
+        for _ in range(2):
+            strides, inner = [0] * dims, 1
+            for axis in ([dims - 1, *torch.randperm(dims - 1, generator=g).tolist()] if pick(0, 1) else range(dims - 1, -1, -1)):
+                strides[axis] = pick(inner, inner, inner, inner + 1, 2 * inner, max(inner - 1, 0), 0, pick(2, 3, 7))
+                inner = max(inner, strides[axis] * shape[axis])
+            if len(views) == 1 and pick(0, 1):
+                strides = list(views[0].stride())
+                shape[-2] = pick(1, 2, 3)
+            views.append(torch.as_strided(buf, shape, strides, pick(0, 0, 1, 2, 6, 12, 30, 31, 64)))
+        a, b = views
+        pa, pb = _places(a), _places(b)
+        assert P._meet(a, b) == bool(set(pa) & set(pb)) == P._meet(b, a)
+        assert P._one_place_each(a) == (len(set(pa)) == len(pa))
+        if dims == 4 and a.shape[:2] == b.shape[:2] and a.shape[3] == b.shape[3]:   # what is seen at once is so
+            d = a.shape[3]
+            if P._side_by_side(*a.shape[:2], a.shape[2], b.shape[2], d, a.element_size(), *(x for t in views for x in (t.data_ptr(), *t.stride()[:3]))) \
+                    and all(d == 1 or t.stride(3) == 1 for t in views):
+                assert not P._meet(a, b) and P._one_place_each(a) and P._one_place_each(b)
+                at_once += 1
+        seen[P._meet(a, b), P._one_place_each(a)] = seen.get((P._meet(a, b), P._one_place_each(a)), 0) + 1
+    assert min(seen.values()) > 100 and len(seen) == 4 and at_once > 20, (seen, at_once)
+
+
+def test_where_large_tensors_lie(P):
+    """Projections of many tokens: queries and keys side by side, one shifted by an element, transposed, in another order."""
+    store = torch.empty(4 * 4096 * 8192, dtype=BF)   # (never touched)
+    view = lambda shape, strides, offset=0: store.as_strided(shape, strides, offset)
+    q, k = view((4, 4096, 32, 128), (4096 * 8192, 8192, 128, 1)), view((4, 4096, 8, 128), (4096 * 8192, 8192, 128, 1), 4096)
+    assert not P._meet(q, k) and not P._meet(k, q) and P._one_place_each(q) and P._one_place_each(k)
+    for a, b in ((q, k), (k, q)):
+        lies = lambda t: (t.data_ptr(), *t.stride()[:3])
+        assert P._side_by_side(4, 4096, a.shape[2], b.shape[2], 128, 2, *lies(a), *lies(b))
+        assert not P._side_by_side(4, 4096, a.shape[2], b.shape[2], 128, 2, *lies(a), a.data_ptr(), *lies(b)[1:])
+    assert P._meet(q, view((4, 4096, 8, 128), (4096 * 8192, 8192, 128, 1), 4095))
+    padded = [view((4, 4096, 16, 48), (4096 * 8192, 8192, 128, 1), at) for at in (0, 48, 2048)]
+    assert not any(P._meet(x, y) for i, x in enumerate(padded) for y in padded[:i])
+    assert P._meet(padded[0], view((4, 4096, 16, 48), (4096 * 8192, 8192, 128, 1), 47))
+    long = view((1, 16384, 32, 128), (0, 8192, 128, 1))
+    assert P._meet(long, q) and not P._meet(long, k)
+    other = view((4, 4096, 8, 128), (8192, 4 * 8192, 128, 1), 4096)   # tokens before the batch
+    assert not P._meet(q, other) and P._meet(k, other) and P._one_place_each(other)
+    assert not P._one_place_each(view((4, 4096, 32, 128), (4096 * 8192, 8192, 127, 1)))
+    square = view((64, 64, 8), (512, 8, 1))
+    assert P._same_view(square, view((64, 64, 8), (512, 8, 1))) and not P._same_view(square, square.transpose(0, 1))
+    assert P._same_view(view((1, 5, 3, 8), (7, 24, 8, 1)), view((1, 5, 3, 8), (120, 24, 8, 1)))
+    raw = torch.empty(40, dtype=torch.uint8)
+    a, b = raw[:16].view(BF), raw[16:32].view(BF)
+    assert not P._meet(a, b) and P._meet(a, raw[14:30].view(BF))

@@ -530,3 +530,33 @@ def test_norm_rotate_of_odd_frequencies(P):
         assert ((got.double().cpu() - want).abs() <= tol + U * want.abs()).all()
     a, _ = P.norm_rotate_qk(q, q, None, None, P.Rotation(f.cuda()), pos.cuda())
     assert a[..., [6, 7, 14, 15]].isnan().all() and a[..., [0, 1, 2, 3, 4, 5, 8, 9, 10, 11, 12, 13]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_norm_rotate_results_that_meet_the_inputs_are_refused(P, ops, dtype):
+    """A transposed view of the input, views an element, a head or a token on, the other's place: refused before any launch.  Side by
+    side in one buffer, and each over its own input: as with new results."""
+    from distributed_xfold_b200._cabi import XfoldError
+    n, d = 6, 8
+    q, k = torch.randn(n, n, d, generator=gen(1)).to(dtype).cuda(), torch.randn(n, 3, d, generator=gen(2)).to(dtype).cuda()
+    new_k = torch.empty_like(k)
+    buf = torch.randn((n + 1) * n * d + 1, generator=gen(3)).to(dtype).cuda()
+    at = lambda off: buf[off:off + n * n * d].view(n, n, d)
+    keep = q.clone(), buf.clone()
+    for q_in, out in ((q, q.transpose(0, 1)), (at(0), at(1)), (at(0), at(d)), (at(0), at(n * d)), (at(n * d), at(0)),
+                      (q, q.as_strided((n, n, d), (d, d, 1)))):
+        with pytest.raises(XfoldError, match="results of queries and keys"):
+            P.norm_rotate_qk(q_in, k, None, None, out=(out, new_k))
+    wide = torch.randn(n, 4, d, generator=gen(4)).to(dtype).cuda()
+    for args in ((wide[:, :3], k, (wide[:, 1:], new_k)), (k, wide[:, :3], (wide[:, 1:], new_k)), (k, q[:, :3], (wide[:, :3], wide[:, 1:])),
+                 (wide[:, :3], wide[:, 1:], (wide[:, :3], wide[:, 1:]))):
+        with pytest.raises(XfoldError, match="results of queries and keys"):
+            P.norm_rotate_qk(*args[:2], None, None, out=args[2])
+    assert torch.equal(q, keep[0]) and torch.equal(buf, keep[1])
+    fused = torch.randn(n, 12, d, generator=gen(5)).to(dtype).cuda()
+    ref = P.norm_rotate_qk(fused[:, :4], fused[:, 4:7], None, None)
+    P.norm_rotate_qk(fused[:, :4], fused[:, 4:7], None, None, out=(fused[:, 8:], fused[:, 4:7]))
+    assert torch.equal(fused[:, 8:], ref[0]) and torch.equal(fused[:, 4:7], ref[1])
+    P.norm_rotate_qk_(fused[:, :4], new_k, None, None)
+    assert torch.equal(fused[:, :4], ref[0])
+    ops.synchronize_and_check()
