@@ -454,6 +454,7 @@ struct QkArgs {
   long long pos_b;
   int B, S, D, rot, log_g;
   float eps;
+  int early;            // the next kernel may start while this one runs
   float* partial;       // backward: [CTAs][D], those of the queries in front
 };
 
@@ -745,7 +746,7 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_kernel(const QkA
   __shared__ __align__(16) uint8_t ring[QK_WARPS][Stream::SMEM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  pdl_launch();
+  if (a.early) pdl_launch();
   const int which = int(blockIdx.x) >= a.t[0].ctas;
   const QkTensor& q = a.t[which];
   QkPlace at[NS];
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_grad_kernel(cons
   __shared__ __align__(16) uint8_t ring[QK_WARPS][Stream::SMEM];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  pdl_launch();
+  if (a.early) pdl_launch();
   const int which = int(blockIdx.x) >= a.t[0].ctas;
   const QkTensor& q = a.t[which];
   QkPlace at[NS];
@@ -949,6 +950,26 @@ static int qk_piece(const QkArgs& a, int elem, bool grad) {
   return V;
 }
 
+// Whether a result has a cache line in common with what the call reads.  Pieces of less than 16 bytes are read through L1 (cp.async
+// past it takes 16), where a line's copy does not learn of what other SMs write to it.  A next kernel on the same SM that started
+// before those writes would read the old numbers: it starts behind the last of them then.
+static bool qk_over_its_inputs(const QkArgs& a, int elem, bool grad) {
+  auto meet = [&](const QkTensor& p, const void* x, long long xb, long long xt, long long xh, const QkTensor& q, const void* y, long long yb, long long yt,
+                  long long yh) {
+    auto lines = [&](const void* at, long long b, long long t, long long h, int H, bool last) {
+      long long off = last ? a.D : 0;
+      const long long reach[3] = {(a.B - 1) * b, (a.S - 1) * t, (H - 1) * h};
+      for (long long r : reach) off += last ? std::max(r, 0ll) : std::min(r, 0ll);
+      return ((long long)(uintptr_t)at + off * elem - (last ? 1 : 0)) >> 7;
+    };
+    return p.H && q.H && lines(x, xb, xt, xh, p.H, false) <= lines(y, yb, yt, yh, q.H, true) && lines(y, yb, yt, yh, q.H, false) <= lines(x, xb, xt, xh, p.H, true);
+  };
+  for (const QkTensor& p : a.t)
+    for (const QkTensor& q : a.t)
+      if (meet(p, p.x, p.xb, p.xt, p.xh, q, q.y, q.yb, q.yt, q.yh) || (grad && meet(p, p.d, p.db, p.dt, p.dh, q, q.y, q.yb, q.yt, q.yh))) return true;
+  return false;
+}
+
 // queries and keys get CTAs by their heads and what a token costs besides (about two passes)
 static int qk_divide(Ctx* c, QkArgs& a, int per_sm, int& grid) {
   const long long tokens = (long long)a.B * a.S;
@@ -992,7 +1013,8 @@ static int launch_qk_one(Ctx* c, QkArgs& a, int neighbours, cudaStream_t st) {
 
 template <bool GRAD>
 static int launch_qk(Ctx* c, QkArgs a, int f32, int neighbours, cudaStream_t st, float* dqw = nullptr, float* dkw = nullptr) {
-  const int V = qk_piece(a, f32 ? 4 : 2, GRAD), slots = (a.D / 2 + V - 1) / V;
+  const int elem = f32 ? 4 : 2, V = qk_piece(a, elem, GRAD), slots = (a.D / 2 + V - 1) / V;
+  a.early = V * elem == 16 || !qk_over_its_inputs(a, elem, GRAD);
   a.log_g = 0;
   while ((1 << a.log_g) < slots && a.log_g < 5) ++a.log_g;
   for (QkTensor& q : a.t) q.passes = (q.H + (32 >> a.log_g) - 1) / (32 >> a.log_g);

@@ -560,3 +560,37 @@ def test_norm_rotate_results_that_meet_the_inputs_are_refused(P, ops, dtype):
     P.norm_rotate_qk_(fused[:, :4], new_k, None, None)
     assert torch.equal(fused[:, :4], ref[0])
     ops.synchronize_and_check()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d,pitch,first", [(24, 24, 0), (24, 26, 0), (24, 24, 1), (48, 48, 4), (6, 6, 0), (64, 64, 0)])
+def test_norm_rotate_in_place_time_after_time(P, ops, d, pitch, first, dtype):
+    """Pieces of all widths in one buffer, each call behind the other, also from a graph: what calls with results of their own give."""
+    g = gen(d + pitch)
+    b, s, hq, hk, rounds = 3, 400, 7, 5, 6
+    start = torch.randn(b, s, first + (hq + hk) * pitch, generator=g).to(dtype).cuda()
+    w = [(1 + 0.2 * torch.randn(d, generator=g)).cuda() for _ in range(2)]
+    r = P.Rotation.make(d)
+
+    def views(buf):
+        return [buf[..., first + i * hq * pitch:first + (hq if i == 0 else hq + hk) * pitch].unflatten(-1, (-1, pitch))[..., :d] for i in range(2)]
+    apart = torch.empty_like(start), torch.empty_like(start)
+    for i in range(rounds):
+        src, dst = (start if i == 0 else apart[(i + 1) % 2]), apart[i % 2]
+        dst.copy_(src)
+        P.norm_rotate_qk(*views(src), *w, r, out=tuple(views(dst)))
+    want = apart[(rounds - 1) % 2]
+    got = start.clone()
+    for _ in range(rounds):
+        P.norm_rotate_qk_(*views(got), *w, r)
+    assert torch.equal(got, want)
+    static, graph = start.clone(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        for _ in range(rounds):
+            P.norm_rotate_qk_(*views(static), *w, r)
+    for _ in range(5):
+        static.copy_(start)
+        graph.replay()
+        assert torch.equal(static, want)
+    ops.synchronize_and_check()
