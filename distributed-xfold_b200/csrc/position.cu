@@ -415,6 +415,8 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
   if (Sq < 0 || Sk < 0 || H < 1 || nb < 1) return fail(c, XFOLD_ERR_ARG, "relative bias: sizes");
   if (nb > 1024 || reach < 0 || reach > 4096) return fail(c, XFOLD_ERR_ARG, "relative bias: up to 1024 buckets and a reach up to 4096");
   if (H > 65535) return fail(c, XFOLD_ERR_ARG, "relative bias: too many heads");
+  // rows and columns are counted in 32 bits, up to 8 SMs' times 256 rows at a time
+  if (std::max(Sq, Sk) > 0x7fffffff - (1 << 20)) return fail(c, XFOLD_ERR_ARG, "relative bias: too many queries or keys");
   if (!lut || (Sq && !qp) || (Sk && !kp)) return fail(c, XFOLD_ERR_ARG, "relative bias: null argument");
   if ((qg != nullptr) != (kg != nullptr) && Sq && Sk) return fail(c, XFOLD_ERR_ARG, "relative bias: groups of queries and keys come together");
   return XFOLD_OK;

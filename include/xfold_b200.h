@@ -252,7 +252,7 @@ int xfold_cross_attention_fwd(xfold_ctx* ctx, const void* q_data, const void* m_
  *   out[h][i][j] = table[b(i, j)][h],  b(i, j) = buckets[clamp(k_pos[j] - q_pos[i], -reach, reach) + reach],
  * or the table's last row where q_group[i] != k_group[j] (both groups or neither; tokens of different chains).
  *   table float32 [num_buckets][H]; buckets int32 [2 * reach + 1], rows of the table (one that names none makes its entries
- *   not a number); positions and groups int32; num_buckets <= 1024, reach <= 4096.
+ *   not a number); positions and groups int32; num_buckets <= 1024, reach <= 4096, Sq and Sk < 2^31 - 2^20.
  *   form: float32 or bf16 [H][Sq][Sk], or the prepared pair bias of the attention core, float16 [H][Sq][pad8(Sk)] times
  *   log2(e) within +-60000, zero behind the last key (what is not a number: -60000). */
 enum { XFOLD_BIAS_F32 = 0, XFOLD_BIAS_BF16 = 1, XFOLD_BIAS_PREPARED = 2 };

@@ -594,3 +594,18 @@ def test_norm_rotate_in_place_time_after_time(P, ops, d, pitch, first, dtype):
         graph.replay()
         assert torch.equal(static, want)
     ops.synchronize_and_check()
+
+
+def test_relative_bias_of_too_many_queries_or_keys(P):
+    """Lengths that rows counted in 32 bits would run past."""
+    from distributed_xfold_b200._cabi import XfoldError
+    table, lut, one = torch.ones(3, 1).cuda(), torch.arange(3, dtype=torch.int32).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    many = torch.empty(2 ** 31 - 1000, dtype=torch.int32, device="cuda")
+    for q, k in ((many, one), (one, many)):
+        with pytest.raises(XfoldError, match="too many queries or keys"):
+            P.relative_position_bias(table, lut, q, k, dtype=BF)
+        with pytest.raises(XfoldError, match="too many queries or keys"):
+            P.relative_position_bias_backward(torch.empty(1, 1, 1, device="cuda").expand(1, q.numel(), k.numel()) if k is one
+                                              else torch.empty(1, 1, k.numel(), dtype=BF, device="cuda"), 3, lut, q, k)
+    del many
+    torch.cuda.empty_cache()
