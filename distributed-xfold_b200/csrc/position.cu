@@ -143,12 +143,14 @@ static void launch_rel_fwd(Ctx* c, RelFwdArgs a, cudaStream_t st) {
   a.log_cx = 0;
   while ((1 << a.log_cx) < chunks && a.log_cx < 8) ++a.log_cx;
   const int cx = 1 << a.log_cx, ry = 256 / cx, gx = (chunks + cx - 1) / cx, gy_most = (a.s.Sq + ry - 1) / ry;
-  // heads of a CTA: as many as 32 KB of table hold, fewer where the SMs would otherwise have nothing to do
-  a.hg = std::max(1, std::min(a.s.H, int(32768 / ((a.s.nb + 2) * sizeof(E)))));
+  // heads of a CTA: as many as 32 KB of table hold (less where the buckets of the longest reach leave less of 48 KB), fewer where
+  // the SMs would otherwise have nothing to do
+  const size_t lut = (2 * a.s.reach + 1) * 2, room = std::min<size_t>(32768, (48 * 1024 - lut) & ~size_t(15));
+  a.hg = std::max(1, std::min(a.s.H, int(room / ((a.s.nb + 2) * sizeof(E)))));
   while (a.hg > 1 && (long long)gx * gy_most * ((a.s.H + a.hg - 1) / a.hg) < c->sm_count) a.hg = (a.hg + 1) / 2;
   const int gz = (a.s.H + a.hg - 1) / a.hg;
   const int gy = (int)std::max(1ll, std::min({(long long)gy_most, 8ll * c->sm_count / std::max(1ll, (long long)gx * gz), 65535ll}));
-  const size_t smem = (((size_t)a.hg * (a.s.nb + 2) * sizeof(E) + 15) & ~size_t(15)) + (2 * a.s.reach + 1) * 2;
+  const size_t smem = (((size_t)a.hg * (a.s.nb + 2) * sizeof(E) + 15) & ~size_t(15)) + lut;
   ProfScope ps(c, XFOLD_K_MASK_BIAS, st);
   launch_pdl(rel_bias_kernel<E, V>, dim3(gx, gy, gz), 256, smem, st, a);
 }

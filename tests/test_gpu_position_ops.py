@@ -609,3 +609,20 @@ def test_relative_bias_of_too_many_queries_or_keys(P):
                                               else torch.empty(1, 1, k.numel(), dtype=BF, device="cuda"), 3, lut, q, k)
     del many
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("form", ["f32", "bf16", "prepared"])
+@pytest.mark.parametrize("nb,heads", [(254, 32), (510, 16), (510, 32), (908, 9), (1022, 8), (1022, 16), (1024, 5)])
+@pytest.mark.parametrize("sk", [264, 257])
+def test_relative_bias_of_the_largest_reach(P, ops, nb, heads, form, sk):
+    g = gen(nb + heads)
+    sq, reach = 700, 4096
+    lut = torch.randint(0, nb, (2 * reach + 1,), generator=g).int()
+    qp, kp = (torch.randint(-4500, 4500, (n,), generator=g).int() for n in (sq, sk))
+    table = torch.randn(nb, heads, generator=g)
+    want = table[lut[(kp.long()[None] - qp.long()[:, None]).clamp(-reach, reach) + reach].long()].permute(2, 0, 1)
+    got = P.relative_position_bias(table.cuda(), lut.cuda(), qp.cuda(), kp.cuda(), dtype=BF if form == "bf16" else F32, prepared=form == "prepared")
+    if form == "prepared":
+        want = (want * 1.4426950408889634).clamp(-60000, 60000).half()
+    assert torch.equal(got[..., :sk].cpu(), want.to(got.dtype))
+    ops.synchronize_and_check()
