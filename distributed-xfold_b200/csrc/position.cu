@@ -438,7 +438,7 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
 // Pieces are 16 bytes where sizes allow it: of 8, sums over twice as many lanes and addresses for half as much work cost more than
 // the fewer registers give back (4 x 4096 tokens, 32 + 8 heads of 128 in 16 bits: 79 and, backward, 137 us).  Warps take ranges of
 // passes that begin and end anywhere in a token, so that none has a token more than another.
-// Now 62 us (5.4 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64: 9.4 and 17.9.  Bound by bytes and the chain of a pass
+// Now 61 us (5.5 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64, half rotated: 9.6 and 18.4.  Bound by bytes and the chain of a pass
 // (sums over the lanes, root); where a head's width is no power of two some lanes idle (80 of 128: 5 of 8 lanes; groups of any
 // size were slower, by their sums).
 // ---------------------------------------------------------------------------------------------
@@ -556,6 +556,9 @@ __device__ __forceinline__ void qk_angles(const QkArgs& a, const unsigned long l
   }
   __syncwarp();
 }
+
+// Of a part of the head that does not rotate: its elements have no partners, whose infinities would become theirs (0 * inf).
+__device__ __forceinline__ bool qk_alone(const QkPlace& pl) { return pl.angle < 0 && pl.pa >= 0; }
 
 // The lane's 2 V elements are V pairs of neighbouring registers.  An element's partner is V elements on (halves), or the other
 // of its pair.
@@ -799,8 +802,13 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_kernel(const QkA
         float2 y[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) x[n][j] = fmul2(x[n][j], make_float2(r, r));  // (first: large elements and weights could overflow)
+        if (qk_alone(at[n])) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] = ffma2(qk_partner<V, NEIGH>(x[n], j), B[n][j], fmul2(x[n][j], A[n][j]));
+          for (int j = 0; j < V; ++j) y[j] = fmul2(x[n][j], A[n][j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[j] = ffma2(qk_partner<V, NEIGH>(x[n], j), B[n][j], fmul2(x[n][j], A[n][j]));
+        }
         if (mine && at[n].pa >= 0) qk_store<T, V>(y, at[n], dst);
       }
       dst += per_pass * q.yh;
@@ -812,7 +820,9 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_kernel(const QkA
 // Backward, with g = the gradient turned back, times the scale, and r = rsqrt(mean(x^2) + eps):
 //   dw_i = sum over tokens and heads of g_i x_i r;  dx = r (g w - x r^2 mean(g w x)).
 // A lane's place in the head is always the same: the weights' gradients are sums in its registers until the end.
-template <typename T, int V, bool NEIGH>
+// PART: some elements do not rotate.  (A kernel of its own: 4 x 4096 tokens, 40 heads of 128, neighbours 90.4 us, and 93.3 where
+// partners of no use are looked for.  Two ways through, as in the forward, which loses nothing by them: 100.9.)
+template <typename T, int V, bool NEIGH, bool PART>
 __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_grad_kernel(const QkArgs a) {
   typedef QkStream<T, V, true> Stream;
   constexpr int NS = qk_slots<V>();
@@ -858,7 +868,11 @@ __global__ void __launch_bounds__(QK_WARPS * 32) qk_norm_rotate_grad_kernel(cons
       for (int n = 0; n < NS; ++n) {
         float2 e[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) e[j] = ffma2(qk_partner<V, NEIGH>(g[n], j), B[n][j], fmul2(g[n][j], A[n][j]));
+        for (int j = 0; j < V; ++j) {
+          float2 partner = qk_partner<V, NEIGH>(g[n], j);
+          if (PART && qk_alone(at[n])) partner = make_float2(0.f, 0.f);
+          e[j] = ffma2(partner, B[n][j], fmul2(g[n][j], A[n][j]));
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           g[n][j] = e[j];
@@ -997,11 +1011,15 @@ static int qk_divide(Ctx* c, QkArgs& a, int per_sm, int& grid) {
 template <typename T, int V, bool GRAD>
 static int launch_qk_one(Ctx* c, QkArgs& a, int neighbours, cudaStream_t st) {
   auto kern = [&] {
-    if constexpr (GRAD) return neighbours ? qk_norm_rotate_grad_kernel<T, V, true> : qk_norm_rotate_grad_kernel<T, V, false>;
-    else return neighbours ? qk_norm_rotate_kernel<T, V, true> : qk_norm_rotate_kernel<T, V, false>;
+    if constexpr (GRAD) {
+      if (a.rot < a.D) return neighbours ? qk_norm_rotate_grad_kernel<T, V, true, true> : qk_norm_rotate_grad_kernel<T, V, false, true>;
+      return neighbours ? qk_norm_rotate_grad_kernel<T, V, true, false> : qk_norm_rotate_grad_kernel<T, V, false, false>;
+    } else {
+      return neighbours ? qk_norm_rotate_kernel<T, V, true> : qk_norm_rotate_kernel<T, V, false>;
+    }
   }();
-  static int per_sm[2] = {0, 0};  // resident CTAs
-  int& n = per_sm[neighbours ? 1 : 0];
+  static int per_sm[4] = {0, 0, 0, 0};  // resident CTAs
+  int& n = per_sm[(neighbours ? 1 : 0) + (a.rot < a.D ? 2 : 0)];
   if (!n) {
     int got = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, QK_WARPS * 32, 0) != cudaSuccess || got < 1)

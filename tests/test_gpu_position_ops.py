@@ -626,3 +626,41 @@ def test_relative_bias_of_the_largest_reach(P, ops, nb, heads, form, sk):
         want = (want * 1.4426950408889634).clamp(-60000, 60000).half()
     assert torch.equal(got[..., :sk].cpu(), want.to(got.dtype))
     ops.synchronize_and_check()
+
+
+def same(got, want):
+    """The same not-a-numbers and infinities."""
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()), (got.isnan() ^ want.isnan()).nonzero()[:5]
+    assert torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf())
+
+
+WHERE = [(24, 0, False), (24, 12, True), (64, 32, False), (64, 16, True), (66, 6, False), (80, 40, False), (128, 64, True), (256, 128, False), (26, 2, True)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d,rot,inter", WHERE)
+@pytest.mark.parametrize("at", [0, -1, -3])
+def test_norm_rotate_keeps_what_is_not_finite_to_its_pair(P, ops, d, rot, inter, dtype, at):
+    g = gen(d + rot)
+    q, k = (torch.randn(2, 5, h, d, generator=g).to(dtype) for h in (3, 2))
+    dq, dk = (torch.randn(x.shape, generator=g).to(dtype) for x in (q, k))
+    qw, kw = (1 + 0.2 * torch.randn(d, generator=g) for _ in range(2))
+    qw[at], kw[at] = float("inf"), float("nan")
+    rotation = P.Rotation.make(rot, interleaved=inter) if rot else None
+    pos = torch.randint(1, 50, (2, 5), generator=g).int()
+    cu = lambda *t: [x.cuda() for x in t]
+    out = P.norm_rotate_qk(*cu(q, k, qw, kw), rotation, pos.cuda())
+    for x, w, o in ((q, qw, out[0]), (k, kw, out[1])):
+        same(o, turned(plain(x, w, None, None, 1e-6, 1.0), rotation, pos))
+    ones = torch.ones(d)
+    x = q.clone()
+    x[0, 1, 0, at], x[1, 2, 2, at] = float("inf"), float("nan")
+    same(P.norm_rotate_qk(*cu(x, k, ones, ones), rotation, pos.cuda())[0], turned(plain(x, None, None, None, 1e-6, 1.0), rotation, pos))
+    y = dq.clone()
+    y[0, 1, 0, at] = float("inf")
+    got = P.norm_rotate_qk_backward(*cu(y, dk, q, k, ones, ones), rotation, pos.cuda())
+    back, x64 = turned(y.double(), rotation, pos, back=True), q.double()
+    r = (x64.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    same(got[2], (back * x64 * r).sum((0, 1, 2)))
+    same(got[0], r * (back - x64 * r * r * (back * x64).mean(-1, keepdim=True)))
