@@ -3,6 +3,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 
 #include "stages.h"
@@ -485,7 +486,7 @@ template <int BN, typename OutT>
 static int launch_i8_one(Ctx* c, const CUtensorMap& tmA, const int8_t* w, long long ldw, I8Args a, cudaStream_t st) {
   using Cfg = I8Cfg<BN>;
   auto kern = i8_gemm_kernel<BN, OutT>;
-  static bool attr_done[8] = {false};
+  static std::atomic<bool> attr_done[8];
   if (!attr_done[c->device & 7]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return fail(c, XFOLD_ERR_LAUNCH, "int8 product: %s", cudaGetErrorString(e));

@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "stages.h"
 #include "umma.cuh"
@@ -399,7 +400,7 @@ static RelBwdPlan rel_bwd_plan(int nb, int H, int Sq, int Sk, int reach, int V, 
 template <typename E, int V, bool VEC>
 static int launch_rel_bwd(Ctx* c, RelBwdArgs a, const RelBwdPlan& p, cudaStream_t st) {
   auto kern = a.s.k_grp ? rel_bias_grad_kernel<E, V, VEC, true> : rel_bias_grad_kernel<E, V, VEC, false>;
-  static bool attr_done[8] = {false};
+  static std::atomic<bool> attr_done[8];
   if (!attr_done[c->device & 7]) {
     cudaError_t e = cudaFuncSetAttribute(rel_bias_grad_kernel<E, V, VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     if (e == cudaSuccess)
@@ -1018,13 +1019,15 @@ static int launch_qk_one(Ctx* c, QkArgs& a, int neighbours, cudaStream_t st) {
       return neighbours ? qk_norm_rotate_kernel<T, V, true> : qk_norm_rotate_kernel<T, V, false>;
     }
   }();
-  static int per_sm[4] = {0, 0, 0, 0};  // resident CTAs
-  int& n = per_sm[(neighbours ? 1 : 0) + (a.rot < a.D ? 2 : 0)];
+  // resident CTAs; contexts in other threads may find them at the same time
+  static std::atomic<int> per_sm[4];
+  std::atomic<int>& known = per_sm[(neighbours ? 1 : 0) + (a.rot < a.D ? 2 : 0)];
+  int n = known.load(std::memory_order_relaxed);
   if (!n) {
     int got = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kern, QK_WARPS * 32, 0) != cudaSuccess || got < 1)
       return fail(c, XFOLD_ERR_LAUNCH, "qk norm: occupancy");
-    n = std::min(got, QK_MOST);
+    known.store(n = std::min(got, QK_MOST), std::memory_order_relaxed);
   }
   int grid = 0;
   if (int rc = qk_divide(c, a, n, grid)) return rc;

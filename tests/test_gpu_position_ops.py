@@ -664,3 +664,43 @@ def test_norm_rotate_keeps_what_is_not_finite_to_its_pair(P, ops, d, rot, inter,
     r = (x64.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
     same(got[2], (back * x64 * r).sum((0, 1, 2)))
     same(got[0], r * (back - x64 * r * r * (back * x64).mean(-1, keepdim=True)))
+
+
+def test_calls_of_two_contexts_in_two_threads(P, ops):
+    """Contexts have locks of their own: what the library keeps for all of them is found by both at once."""
+    import ctypes
+    import threading
+    from distributed_xfold_b200._cabi import QK_NORM, load
+    lib, handles = load(), [ctypes.c_void_p() for _ in range(2)]
+    for h in handles:
+        assert lib.xfold_ctx_create(0, ctypes.byref(h)) == 0
+    shapes = [(d, rot, dt) for d in (6, 20, 40, 128) for rot in (d, d // 4 * 2) for dt in (BF, F32)]
+    work = []
+    for d, rot, dt in shapes:
+        q, k = torch.randn(2, 30, 5, d, generator=gen(d)).to(dt).cuda(), torch.randn(2, 30, 3, d, generator=gen(d + 1)).to(dt).cuda()
+        r = P.Rotation.make(rot)
+        work.append((q, k, r, P.norm_rotate_qk(q, k, None, None, r), [[torch.empty_like(t) for t in (q, k)] for _ in handles]))
+    torch.cuda.synchronize()
+    gate, wrong = threading.Barrier(2, timeout=60), []
+
+    def go(i):
+        stream = torch.cuda.Stream()
+        for q, k, r, _, outs in work:
+            heads = lambda t: (t.data_ptr(), *t.stride()[:3])
+            desc = QK_NORM.pack(2, 30, 5, 3, q.shape[-1], 2 * r.freqs.numel(), 0, q.dtype is F32, 0, 0, r.freqs.data_ptr(), 0, 0, 1e-6, 1.0,
+                                *heads(q), *heads(k), *heads(outs[i][0]), *heads(outs[i][1]), *[0] * 8)
+            gate.wait()
+            if lib.xfold_qk_norm_rotate_fwd(handles[i], desc, stream.cuda_stream):
+                wrong.append(i)
+        stream.synchronize()
+    threads = [threading.Thread(target=go, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for _, _, _, want, outs in work:
+        for out in outs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    for h in handles:
+        lib.xfold_ctx_destroy(h)
