@@ -259,6 +259,7 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
+constexpr int I8_MOST_K = 131072;  // sums from -127 * 128 K to 128 * 128 K
 constexpr int I8_BM = 128, I8_BK = 128, I8_THREADS = 320;
 constexpr uint32_t I8_OUT_WARP = 4096;  // staging of an epilogue warp: two [32][32] tiles of 16 bits or one of 32
 
@@ -410,6 +411,10 @@ i8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         float v[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = float(int(r[e]));
+        if (p.K == I8_MOST_K) {  // products of -128 alone: their sum, 2^31, is the one that wraps around, to what no other sum is
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = r[e] == 0x80000000u ? 2147483648.f : v[e];
+        }
         // the store that last used this staging tile must have read it out
         if constexpr (F32) tma_store_wait_read<0>();
         else tma_store_wait_read<1>();
@@ -668,8 +673,7 @@ static int launch_i8_rows(Ctx* c, const RowsArgs& a, cudaStream_t st) {
 
 static int i8_check(Ctx* c, long long M, int K, int N) {
   if (M < 0 || K < 1 || N < 0) return fail(c, XFOLD_ERR_ARG, "int8 linear: sizes");
-  // 127 * 127 * K stays within the 32-bit sums
-  if (K > 131072) return fail(c, XFOLD_ERR_ARG, "int8 linear: K up to 131072");
+  if (K > I8_MOST_K) return fail(c, XFOLD_ERR_ARG, "int8 linear: K up to 131072");
   if (M >= (1ll << 31) - 128 || N >= (1 << 30)) return fail(c, XFOLD_ERR_ARG, "int8 linear: too many rows");
   return XFOLD_OK;
 }

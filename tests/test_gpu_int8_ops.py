@@ -318,3 +318,15 @@ def test_one_number_broadcast_over_the_rows(Q, ops, dtype):
         assert (q == -127).all() and torch.equal(s, Q.quantize_rows(x)[1].expand(m))
         assert torch.equal(Q.linear_int8(wide, w, ws), Q.linear_int8(wide.contiguous(), w, ws))
     ops.synchronize_and_check()
+
+
+@pytest.mark.parametrize("m", [1, 4, 40, 200])
+def test_linear_int8_of_the_largest_products(Q, ops, m):
+    k, n = 131072, 70
+    x = torch.full((m, k), -128, dtype=I8)
+    x[1::2, ::5] = 127
+    w = torch.full((n, k), -128, dtype=I8)
+    w[1::2, 1::3] = 127
+    out = Q.linear_int8_quantized(x.cuda(), torch.ones(m).cuda(), w.cuda(), torch.ones(n).cuda(), dtype=F32)
+    want = x.double() @ w.double().T
+    assert want[0, 0] == 2.0 ** 31 and torch.equal(out.cpu(), want.float())
