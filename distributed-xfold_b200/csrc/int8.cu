@@ -259,6 +259,16 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
+// sum * rs * ws + bias.  The scales' product first: a sum times a large scale alone could overflow.  Where that product is subnormal
+// and would lose bits, or beyond all numbers and not to be had by a sum of 0, the larger scale first: in the one case it is less than
+// 2^23, in the other no result but 0 is a number.
+__device__ __forceinline__ float i8_scaled(float sum, float rs, float ws, float bias) {
+  const float p = rs * ws;
+  if (fabsf(p) >= FLT_MIN && fabsf(p) <= FLT_MAX) return fmaf(sum, p, bias);
+  const bool row = fabsf(rs) > fabsf(ws);
+  return fmaf(sum * (row ? rs : ws), row ? ws : rs, bias);
+}
+
 constexpr int I8_MOST_K = 131072;  // sums from -127 * 128 K to 128 * 128 K
 constexpr int I8_BM = 128, I8_BK = 128, I8_THREADS = 320;
 constexpr uint32_t I8_OUT_WARP = 4096;  // staging of an epilogue warp: two [32][32] tiles of 16 bits or one of 32
@@ -407,6 +417,11 @@ i8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         uint8_t* so = F32 ? stage_out : stage_out + (ochunk & 1u) * (I8_OUT_WARP / 2);
         uint32_t r[32];
         tmem_ld32(taddr + c * 64 + ch * 32, r);
+        // whether a scale of the columns (zero aside) and a row's make a product that i8_scaled has to look at
+        const uint32_t size = __float_as_uint(fabsf(cs));
+        const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, size ? size : 0x7f800000u)),
+                    most = __uint_as_float(__reduce_max_sync(0xffffffffu, size));
+        const bool odd = __any_sync(0xffffffffu, rs != 0.f && !(fabsf(rs) * least >= FLT_MIN && fabsf(rs) * most <= FLT_MAX));
         tmem_ld_wait();
         float v[32];
 #pragma unroll
@@ -425,13 +440,25 @@ i8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         sv[32 + lane] = cs;
         __syncwarp();
         if (c + 1 < nch) fetch_cols(c + 1);
-#pragma unroll  // (the scales' product first: a sum times a large scale of its row alone could overflow)
-        for (int e = 0; e < 8; ++e) {
-          const float4 fb = reinterpret_cast<const float4*>(sv)[e], fs = reinterpret_cast<const float4*>(sv)[8 + e];
-          v[4 * e] = fmaf(v[4 * e], rs * fs.x, fb.x);
-          v[4 * e + 1] = fmaf(v[4 * e + 1], rs * fs.y, fb.y);
-          v[4 * e + 2] = fmaf(v[4 * e + 2], rs * fs.z, fb.z);
-          v[4 * e + 3] = fmaf(v[4 * e + 3], rs * fs.w, fb.w);
+        const float4 *fb = reinterpret_cast<const float4*>(sv), *fs = fb + 8;
+        if (!odd) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 b = fb[e], f = fs[e];
+            v[4 * e] = fmaf(v[4 * e], rs * f.x, b.x);
+            v[4 * e + 1] = fmaf(v[4 * e + 1], rs * f.y, b.y);
+            v[4 * e + 2] = fmaf(v[4 * e + 2], rs * f.z, b.z);
+            v[4 * e + 3] = fmaf(v[4 * e + 3], rs * f.w, b.w);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 b = fb[e], f = fs[e];
+            v[4 * e] = i8_scaled(v[4 * e], rs, f.x, b.x);
+            v[4 * e + 1] = i8_scaled(v[4 * e + 1], rs, f.y, b.y);
+            v[4 * e + 2] = i8_scaled(v[4 * e + 2], rs, f.z, b.z);
+            v[4 * e + 3] = i8_scaled(v[4 * e + 3], rs, f.w, b.w);
+          }
         }
         __syncwarp();
         if constexpr (F32) {
@@ -650,7 +677,7 @@ __global__ void __launch_bounds__(256) i8_rows_kernel(const RowsArgs a) {
     }
   const int n = n0 + lane / MB, r = lane % MB;
   if (lane < ROWS_C * MB && n < a.N && r < M) {
-    const float y = fmaf(float(mine), scale[r] * a.w_scale[n], a.bias ? a.bias[n] : 0.f);
+    const float y = i8_scaled(float(mine), scale[r], a.w_scale[n], a.bias ? a.bias[n] : 0.f);
     if (a.out_f32) static_cast<float*>(a.out)[r * a.ldo + n] = y;
     else static_cast<bf16*>(a.out)[r * a.ldo + n] = __float2bfloat16(y);
   }

@@ -330,3 +330,35 @@ def test_linear_int8_of_the_largest_products(Q, ops, m):
     out = Q.linear_int8_quantized(x.cuda(), torch.ones(m).cuda(), w.cuda(), torch.ones(n).cuda(), dtype=F32)
     want = x.double() @ w.double().T
     assert want[0, 0] == 2.0 ** 31 and torch.equal(out.cpu(), want.float())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k,n", [(1, 100, 70), (3, 40, 9), (40, 100, 70), (300, 333, 257)])
+@pytest.mark.parametrize("sx,sw", [(2.0 ** -100, 2.0 ** -40), (2.0 ** -30, 2.0 ** -105), (1e-25, 1e-20), (1e-38, 1.7e-4), (2.0 ** -130, 2.0 ** 3), (1e30, 1e-30), (1e-20, 1e25)])
+def test_linear_int8_of_small_scales(Q, ops, m, k, n, sx, sw, dtype):
+    g = gen(m + k)
+    x = torch.randint(-127, 128, (m, (k + 15) // 16 * 16), generator=g).to(I8)[:, :k]
+    w, _ = weights(n, k, 3)
+    xs, ws = (torch.rand(m, generator=g) + 0.5) * sx, (torch.rand(n, generator=g) + 0.5) * sw
+    out = Q.linear_int8_quantized(x.cuda() if k % 16 == 0 else torch.nn.functional.pad(x, (0, -k % 16)).cuda()[:, :k], xs.cuda(), w, ws.cuda(), dtype=dtype)
+    want = (x.double() @ w.cpu().double().T) * xs.double()[:, None] * ws.double()
+    tol = 4 * U * want.abs() + 2.0 ** -149
+    tol = tol + HALF[dtype] * (want.abs() + tol) + (2.0 ** -134 if dtype == BF else 0)
+    err = (out.double().cpu() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 70), (3, 64, 9), (40, 64, 70), (300, 320, 257)])
+@pytest.mark.parametrize("sx,sw", [(1e30, 1e30), (3e38, 2.0), (2.0 ** 100, 2.0 ** 27), (1e20, -1e20)])
+def test_linear_int8_of_large_scales(Q, ops, m, k, n, sx, sw, dtype):
+    """Scales whose product is beyond all numbers: a sum of 0 is 0 all the same, others overflow by their sign."""
+    g = gen(m + k)
+    x, w = (torch.randint(-2, 3, (r, k), generator=g).to(I8) for r in (m, n))
+    x[:, 8:], w[1::2, 3:] = 0, 0
+    bias = torch.randn(n, generator=g)
+    out = Q.linear_int8_quantized(x.cuda(), torch.full((m,), sx).cuda(), w.cuda(), torch.full((n,), sw).cuda(), bias.cuda(), dtype=dtype).float().cpu()
+    sums = (x.double() @ w.double().T)
+    assert (sums == 0).any() and (sums > 0).any() and (sums < 0).any()
+    want = (sums * (float(torch.tensor(sx)) * float(torch.tensor(sw))) + bias.double()).float().to(dtype).float()
+    assert torch.equal(out, want)
