@@ -756,8 +756,8 @@ int xfold_linear_int8_quantized_fwd(xfold_ctx* cx, const void* x, long long ldx,
   if (int rc = i8_check(c, M, K, N)) return rc;
   if (!M || !N) return XFOLD_OK;
   DeviceGuard dev(c);
-  return i8_product(c, (const int8_t*)x, ldx, x_scale, M, K, (const int8_t*)w, ldw, N, w_scale, bias, out, out_is_f32, ldo, c->static_weights,
-                    (cudaStream_t)stream);
+  return i8_product(c, (const int8_t*)x, ldx, x_scale, M, K, (const int8_t*)w, ldw, N, w_scale, bias, out, out_is_f32, ldo, 0,
+                    (cudaStream_t)stream);  // (the kernel before may have made the weights)
 }
 
 size_t xfold_linear_int8_workspace_bytes(long long M, int K) {
