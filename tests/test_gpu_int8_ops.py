@@ -362,3 +362,53 @@ def test_linear_int8_of_large_scales(Q, ops, m, k, n, sx, sw, dtype):
     assert (sums == 0).any() and (sums > 0).any() and (sums < 0).any()
     want = (sums * (float(torch.tensor(sx)) * float(torch.tensor(sw))) + bias.double()).float().to(dtype).float()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 200])
+@pytest.mark.parametrize("k", [1, 15, 33, 1000, 1023])
+def test_products_of_rows_with_numbers_behind_them(Q, m, k):
+    """Rows of both operands whose bytes up to the next row are not zero: none of them is in a sum."""
+    pitch, g = (k + 15) // 16 * 16 + 16, gen(k)
+    wide = [torch.randint(1, 128, (n, pitch), generator=g).to(I8) for n in (m, 70)]
+    x, w = (t.cuda()[:, :k] for t in wide)
+    out = Q.linear_int8_quantized(x, torch.ones(m).cuda(), w, torch.ones(70).cuda(), dtype=F32)
+    want = wide[0][:, :k].double() @ wide[1][:, :k].double().T
+    assert float(want.max()) < 2 ** 24 and torch.equal(out.double().cpu(), want)
+
+
+def test_attention_over_what_the_operators_make(Q, ops):
+    """A layer as a user writes it around them: 8-bit projection to queries, keys and values, norms and rotation where they lie, the
+    bias of two chains; logits, softmax and sum over the values in 64 bits, against the same of 64-bit norms and rotation.
+
+    A query's or key's element is off by its rounding (half a step of bf16 and below 32 u of its pair's length), a logit by at most the
+    sum of those times the other's, d; then a weight of the softmax by a factor within exp(-2 d) and exp(2 d)."""
+    import test_gpu_position_ops as T
+    from distributed_xfold_b200 import position_ops as P
+    n, c, heads, d = 70, 384, 16, 24
+    g = gen(8)
+    x = torch.randn(2, n, c, generator=g).to(BF).cuda()
+    w8, ws = Q.quantize_rows((torch.randn(3 * c, c, generator=g) * c ** -0.5).cuda())
+    proj = Q.linear_int8(x, w8, ws)
+    check_linear(proj, *plain_rows(x), w8, ws, None, BF)
+    q, k, v = (proj[..., i * c:(i + 1) * c].unflatten(-1, (heads, d)) for i in range(3))
+    qw, kw = ((1 + 0.1 * torch.randn(d, generator=g)).cuda() for _ in range(2))
+    rotation, pos = P.Rotation.make(d), torch.arange(n, dtype=torch.int32).cuda()
+    chain, table = (torch.arange(n) // 40).int().cuda(), torch.randn(66, heads, generator=g).cuda()
+    lut = torch.tensor(P.clipped_buckets(32), dtype=torch.int32).cuda()
+    at = torch.arange(n).expand(2, -1)
+    plain = [T.plain(t, w, None, None, 1e-6, f) for t, w, f in ((q, qw, d ** -0.5), (k, kw, 1.0))]
+    want = [T.turned(y, rotation, at) for y in plain]
+    off = [32 * U * T.pair_length(y, rotation) for y in plain]
+    off = [e + HALF[BF] * (y.abs() + e) for e, y in zip(off, want)]
+    P.norm_rotate_qk_(q, k, qw, kw, rotation, pos, q_scale=d ** -0.5)
+    bias = P.relative_position_bias(table, lut, pos, None, chain, chain).double().cpu()
+    b = (torch.arange(n)[None] - torch.arange(n)[:, None]).clamp(-32, 32) + 32
+    assert torch.equal(bias, table.cpu().double()[torch.where(chain.cpu()[:, None] == chain.cpu(), b, 65)].permute(2, 0, 1))
+    dot = lambda a, e: torch.einsum("bihd,bjhd->bhij", a, e)
+    attend = lambda a, e: torch.softmax(dot(a, e) + bias, -1)
+    out = torch.einsum("bhij,bjhd->bihd", attend(q.double().cpu(), k.double().cpu()), v.double().cpu())
+    p = attend(*want)
+    ref, mass = (torch.einsum("bhij,bjhd->bihd", p, t) for t in (v.double().cpu(), v.double().cpu().abs()))
+    worst = (dot(off[0], want[1].abs() + off[1]) + dot(want[0].abs(), off[1])).amax(-1).permute(0, 2, 1)[..., None]
+    assert ((out - ref).abs() <= torch.expm1(2 * worst) * mass + 1e-12).all() and float(worst.max()) < 0.1
+    ops.synchronize_and_check()

@@ -704,3 +704,32 @@ def test_calls_of_two_contexts_in_two_threads(P, ops):
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
     for h in handles:
         lib.xfold_ctx_destroy(h)
+
+
+@pytest.mark.parametrize("case", [c for c in RANGES if not (c[2] and c[3])])
+def test_norm_rotate_of_many_tokens_on_one_side(P, ops, case):
+    """Queries without keys, and keys without queries, over many tokens."""
+    b, s, hq, hk, d, rot, inter, dtype = case
+    q, k, qw, kw, rotation, pos = qk_case(P, b, s, hq, hk, d, rot, inter, dtype, -20, seed=3)
+    out = P.norm_rotate_qk(q, k, qw, kw, rotation, pos.cuda(), q_scale=0.25)
+    for x, w, f, got in ((q, qw, 0.25, out[0]), (k, kw, 1.0, out[1])):
+        assert got.shape == x.shape
+        if x.numel():
+            check_forward(P, x, x, w, w, rotation, pos, pos, 1e-6, f, (got, P.norm_rotate_qk(x, x, w, w, rotation, pos.cuda(), q_scale=f)[1]))
+    ops.synchronize_and_check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("reach", [0, 2, 500])
+def test_relative_bias_gradient_of_far_and_extreme_positions(P, ops, dtype, reach):
+    """Positions at both ends of 32 bits, next to ordinary ones, in eights and in blocks of columns."""
+    g = gen(reach)
+    ends = torch.tensor([-2 ** 31, -2 ** 31 + 1, -2 ** 31 + 400, -7, 0, 5, 2 ** 31 - 400, 2 ** 31 - 2, 2 ** 31 - 1])
+    qp, kp = (ends[torch.randint(0, len(ends), (n,), generator=g)].sort().values.int() for n in (50, 300))
+    nb = 2 * reach + 1
+    b = (kp.long()[None] - qp.long()[:, None]).clamp(-reach, reach) + reach
+    grad = torch.randint(-4, 5, (2, 50, 300), generator=g).to(dtype)
+    got = P.relative_position_bias_backward(grad.cuda(), nb, torch.arange(nb, dtype=torch.int32).cuda(), qp.cuda(), kp.cuda())
+    want = torch.zeros(2, nb, dtype=F64).index_add_(1, b.flatten(), grad.flatten(1).double()).T
+    assert torch.equal(got.double().cpu(), want)
+    ops.synchronize_and_check()
