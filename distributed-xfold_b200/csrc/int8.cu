@@ -242,8 +242,8 @@ static int launch_quantise(Ctx* c, const void* x, int f32, long long ldx, long l
 //   warp 0      : TMA producer, 128-byte-swizzled K-major tiles of 128 bytes along K
 //   warp 1      : tcgen05.mma issuer; owns the tensor memory (2 accumulators)
 //   warps 2..9  : epilogue: scales, bias, rounding; each warp's 32 x 32 parts leave through its own staging tiles
-// 8192 x 4096 x 4096: 94 us, 2.9 PTOP/s (twice what the library's bf16 product reaches); bound by the tensor cores and the operands'
-// trip from L2.  Rows that start in the middle of a sector cost a third of it (5000^3: 103 us at rows 5056 bytes apart, 143 at
+// 8192 x 4096 x 4096: 96 us at 1965 MHz, 2.9 PTOP/s (the library's 91), and 111 (105) where the power limit holds the clock at 1.4
+// GHz; bound by the tensor cores and the operands' trip from L2.  Rows that start in the middle of a sector cost a third of it (5000^3: 103 us at rows 5056 bytes apart, 143 at
 // 5008).  Clusters that share K of one tile, as gemm_split_kernel's, were slower at most sizes.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void umma_i8_if(uint32_t go, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -561,8 +561,9 @@ static int launch_i8(Ctx* c, const int8_t* x, long long ldx, const float* x_scal
 // ---------------------------------------------------------------------------------------------
 // Few rows (a decoding step): bound by the weights, which are read once, 16 bytes to a lane, two channels to a warp, straight
 // into the dot products of four bytes.  With one or two rows every CTA quantises them for itself while its weights are on their
-// way, and the whole layer is one launch.  (4096 x 4096, weights from memory: one row 6.1 us, by quantise_rows_kernel and the
-// tensor cores' tiles, of which there are but 64, 13.4; four rows, quantised before, 6.6 against 12.1; of eight rows the dot products take as long as the tiles.)
+// way, and the whole layer is one launch.  (4096 x 4096, weights from memory: one row 6.7 us, by quantise_rows_kernel and the
+// tensor cores' tiles, of which there are but 64, 13.4; four rows, quantised before, 6.6 against 12.1; of eight rows the dot products
+// take as long as the tiles.)
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_MOST = 4, ROWS_SMEM = 48 * 1024 - 1024;  // rows; bytes of quantised rows in shared memory
 constexpr int ROWS_C = 2, ROWS_U = 4;                       // channels of a warp; pieces of each that a lane has on their way

@@ -439,7 +439,7 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
 // Pieces are 16 bytes where sizes allow it: of 8, sums over twice as many lanes and addresses for half as much work cost more than
 // the fewer registers give back (4 x 4096 tokens, 32 + 8 heads of 128 in 16 bits: 79 and, backward, 137 us).  Warps take ranges of
 // passes that begin and end anywhere in a token, so that none has a token more than another.
-// Now 61 us (5.5 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64, half rotated: 9.6 and 18.4.  Bound by bytes and the chain of a pass
+// Now 61 us (5.5 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64, half rotated: 9.6 and 18.8.  Bound by bytes and the chain of a pass
 // (sums over the lanes, root); where a head's width is no power of two some lanes idle (80 of 128: 5 of 8 lanes; groups of any
 // size were slower, by their sums).
 // ---------------------------------------------------------------------------------------------
@@ -534,7 +534,8 @@ __device__ __forceinline__ QkPlace qk_place(const QkArgs& a, int sl) {
 }
 
 // An angle's whole turns are of no interest, so turns for each position are kept as a fraction of 64 bits (once for a CTA), and
-// their product with the position as one that wraps around: exact but for the fraction's last bit, times the position.  The lowest
+// their product with the position as one that wraps around, without another rounding.  The fraction is as good as the frequency's
+// 53 bits and their product with 1 / (2 pi) (2^-55 of a turn at about one radian), and off by that times the position.  The lowest
 // of them stands for a frequency that is not finite (of half a turn the next is as good).
 constexpr unsigned long long NO_ANGLE = 1ull << 63;
 __device__ __forceinline__ void qk_turns_of_a_position(const QkArgs& a, unsigned long long* turns) {

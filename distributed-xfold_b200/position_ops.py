@@ -1,7 +1,8 @@
 """Positions in attention: a learned bias of the logits by buckets of relative position (with the gradient of its table), and
 the norms of queries and keys for each head together with their rotation by position (with their gradients).
 
-Like the rest of the package these calls are not part of an autograd graph: the backward of each is a call of its own.
+Like the rest of the package these calls are not part of an autograd graph, whether their inputs require gradients or not: the
+backward of each is a call of its own, which a user's ``torch.autograd.Function`` may make.
 """
 from __future__ import annotations
 
@@ -89,7 +90,8 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, q_pos: to
 
     Returns [H, queries, keys] in float32 or bfloat16, or ``prepared``: float16 [H, queries, pad8(keys)] times log2(e), what
     ``ops.attention_pair_bias_core`` takes (as from ``ops.prepare_pair_bias``).  A bucket that names no row of the table makes
-    its entries not a number."""
+    its entries not a number.  In the prepared form numbers end at +-60000, and what is not a number is -60000, as in
+    ``ops.prepare_pair_bias``: such a key is masked, and no error shows."""
     if k_pos is None:
         k_pos, k_group = q_pos, (q_group if k_group is None else k_group)
     if table.dtype is not F32 or table.dim() != 2 or not table.is_contiguous():
