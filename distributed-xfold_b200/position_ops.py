@@ -292,10 +292,20 @@ def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and _axes(a) == _axes(b)
 
 
-def _check_results(q, k, qo, ko, dev) -> None:
-    for o, x in ((qo, q), (ko, k)):
-        if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
-            _refuse("results of queries and keys: shape, type and device of their inputs")
+def _result(o: torch.Tensor, x: torch.Tensor, dev: int, name: str) -> Tuple[int, int, int, int]:
+    if o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev:
+        _refuse("results of queries and keys: shape, type and device of their inputs")
+    return _heads(o, name)
+
+
+def _check_results(q, k, qo, ko, sizes, at_q, at_k, at_qo, at_ko) -> None:
+    """Refuses results without a place for each element, or that meet what is read."""
+    b, s, hq, hk, d, size = sizes
+    if _side_by_side(*sizes, *at_qo, *at_ko) and (
+            at_ko == at_k or _side_by_side(*sizes, *at_qo, *at_k) and _side_by_side(b, s, hk, hk, d, size, *at_ko, *at_k)) and (
+            at_qo == at_q or _side_by_side(*sizes, *at_q, *at_ko) and _side_by_side(b, s, hq, hq, d, size, *at_qo, *at_q)):
+        return
+    for o in (qo, ko):
         if not _one_place_each(o):
             _refuse("results of queries and keys: one place for each element")
     if _meet(qo, ko) or _meet(qo, k) or _meet(ko, q) or any(not _same_view(o, x) and _meet(o, x) for o, x in ((qo, q), (ko, k))):
@@ -317,14 +327,16 @@ def norm_rotate_qk(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
     int32 [tokens] or [batch, tokens] (None: 0, 1, ...).  Results are new, or written to ``out``, each of which may be
     its own input (the same view of it) and otherwise lies apart from the inputs and from the other."""
     dev, n = _qk_norm(q, k, q_weight, k_weight, rotation, positions, eps, q_scale)
+    at = n[-8:]   # where queries, keys and results lie
     if out is None:
         qo, ko = _new(q), _new(k)
+        at += _heads(qo, "") + _heads(ko, "")
     else:
         qo, ko = out
-        if not (qo is q and ko is k and _side_by_side(*n[:5], 4 if n[7] else 2, *n[-8:])):
-            _check_results(q, k, qo, ko, dev)
-    rc = load().xfold_qk_norm_rotate_fwd(ctx(dev), QK_NORM.pack(*n, *_heads(qo, "result of the queries"), *_heads(ko, "result of the keys"),
-                                                                0, 0, 0, 0, 0, 0, 0, 0), _stream(dev))
+        if qo is not q or ko is not k:
+            at += _result(qo, q, dev, "result of the queries") + _result(ko, k, dev, "result of the keys")
+        _check_results(q, k, qo, ko, n[:5] + (4 if n[7] else 2,), at[:4], at[4:8], at[-8:-4], at[-4:])
+    rc = load().xfold_qk_norm_rotate_fwd(ctx(dev), QK_NORM.pack(*n, *at[-8:], 0, 0, 0, 0, 0, 0, 0, 0), _stream(dev))
     check(rc, dev, "xfold_qk_norm_rotate_fwd")
     return qo, ko
 
