@@ -243,8 +243,8 @@ static int launch_quantise(Ctx* c, const void* x, int f32, long long ldx, long l
 //   warp 1      : tcgen05.mma issuer; owns the tensor memory (2 accumulators)
 //   warps 2..9  : epilogue: scales, bias, rounding; each warp's 32 x 32 parts leave through its own staging tiles
 // 8192 x 4096 x 4096: 96 us at 1965 MHz, 2.9 PTOP/s (the library's 91), and 111 (105) where the power limit holds the clock at 1.4
-// GHz; bound by the tensor cores and the operands' trip from L2.  Rows that start in the middle of a sector cost a third of it (5000^3: 103 us at rows 5056 bytes apart, 143 at
-// 5008).  Clusters that share K of one tile, as gemm_split_kernel's, were slower at most sizes.
+// GHz; bound by the tensor cores and the operands' trip from L2.  Rows that start in the middle of a sector cost a third of it
+// (5000^3: 103 us at rows 5056 bytes apart, 143 at 5008).  Clusters that share K of one tile, as gemm_split_kernel's, were slower at most sizes.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ void umma_i8_if(uint32_t go, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(

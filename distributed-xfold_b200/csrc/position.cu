@@ -418,7 +418,7 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
   if (Sq < 0 || Sk < 0 || H < 1 || nb < 1) return fail(c, XFOLD_ERR_ARG, "relative bias: sizes");
   if (nb > 1024 || reach < 0 || reach > 4096) return fail(c, XFOLD_ERR_ARG, "relative bias: up to 1024 buckets and a reach up to 4096");
   if (H > 65535) return fail(c, XFOLD_ERR_ARG, "relative bias: too many heads");
-  // rows and columns are counted in 32 bits, up to 8 SMs' times 256 rows at a time
+  // rows are counted in 32 bits, all CTAs' at a time (eight for each SM, of up to 256 rows)
   if (std::max(Sq, Sk) > 0x7fffffff - (1 << 20)) return fail(c, XFOLD_ERR_ARG, "relative bias: too many queries or keys");
   if (!lut || (Sq && !qp) || (Sk && !kp)) return fail(c, XFOLD_ERR_ARG, "relative bias: null argument");
   if ((qg != nullptr) != (kg != nullptr) && Sq && Sk) return fail(c, XFOLD_ERR_ARG, "relative bias: groups of queries and keys come together");
@@ -439,8 +439,8 @@ static int rel_check(Ctx* c, int nb, int H, int reach, int Sq, int Sk, const voi
 // Pieces are 16 bytes where sizes allow it: of 8, sums over twice as many lanes and addresses for half as much work cost more than
 // the fewer registers give back (4 x 4096 tokens, 32 + 8 heads of 128 in 16 bits: 79 and, backward, 137 us).  Warps take ranges of
 // passes that begin and end anywhere in a token, so that none has a token more than another.
-// Now 61 us (5.5 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64, half rotated: 9.6 and 18.8.  Bound by bytes and the chain of a pass
-// (sums over the lanes, root); where a head's width is no power of two some lanes idle (80 of 128: 5 of 8 lanes; groups of any
+// Now 61 us (5.5 TB/s), backward 99 (5.1); 2 x 2048 tokens, 32 heads of 64, half rotated: 9.6 and 18.8.  Bound by bytes and the
+// chain of a pass (sums over the lanes, root); where a head's width is no power of two some lanes idle (80 of 128: 5 of 8 lanes; groups of any
 // size were slower, by their sums).
 // ---------------------------------------------------------------------------------------------
 struct QkTensor {

@@ -359,8 +359,8 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 //     this kernel, and this kernel for the tensor memory) and after pdl_wait(): L1 is invalidated when a kernel starts, and
 //     a kernel two places ahead must not start while this kernel's predecessor still reads what this kernel overwrites;
 //   * no kernel reads through L1 a buffer that it also writes (or it leaves pdl_launch() out, and its successor starts behind
-//     its last write: norms and rotation in place, with pieces of less than 16 bytes), and no pointer to activations is const __restrict__: the
-//     compiler treats such loads as invariant and may move them above pdl_wait().
+//     its last write: norms and rotation in place, with pieces of less than 16 bytes), and no pointer to
+//     activations is const __restrict__: the compiler treats such loads as invariant and may move them above pdl_wait().
 // ------------------------------------------------------------------------------------
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

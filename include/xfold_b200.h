@@ -272,7 +272,8 @@ int xfold_relative_bias_bwd(xfold_ctx* ctx, const void* grad, int is_f32, long l
  *   y = x * rsqrt(mean(x^2) + eps) * weight (* q_scale for queries); of the first `rot` elements of a head the pairs (a, b),
  *   (i, i + rot / 2) or neighbours (2 i, 2 i + 1), become (a cos t - b sin t, b cos t + a sin t), t = position * freqs[i].
  * Heads of D <= 256 elements (even); batch, token and head strides in elements, so that q and k may lie in the result of a
- * fused projection; a result may lie over its own input (the same strides), and otherwise lies apart from q and k.  weights float32 [D] or NULL (ones); freqs float64 [rot / 2] on the
+ * fused projection; a result may lie over its own input (the same strides), and otherwise lies apart from q, k and the other
+ * result.  weights float32 [D] or NULL (ones); freqs float64 [rot / 2] on the
  * device; positions int32, that of token s of batch entry b at b * pos_batch_stride + s, or NULL (s).  bf16 or float32. */
 typedef struct {
   const void* at; /* (results are written) */
